@@ -175,6 +175,14 @@ def _operands(input, weight, bias, target):
     return input, weight.contiguous(), None if bias is None else bias.contiguous(), target.contiguous(), geometry
 
 
+def _saved_for(layout, input, geometry, weight, bias, target, ignore_index, reduction, saved):
+    """What the forward call left for these operands; computed again if its operands lay differently in
+    memory (``layout``: their geometry and the weight's alignment, on which kernel and contents depend)."""
+    if layout == (geometry, weight.data_ptr() % 16):
+        return saved.contiguous()
+    return xent_forward_(input, geometry, weight, bias, target, ignore_index, reduction, True)[1]
+
+
 class LinearCrossEntropyFunction(torch.autograd.Function):
     """With few labels over float32 images or volumes the gradients are computed in the forward pass,
     with the loss: x, which everything is bound by, is then read once instead of twice.  The
@@ -185,9 +193,9 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
     def forward(ctx, input, weight, bias, target, ignore_index, reduction):
         input, weight, bias, target, geometry = _operands(input, weight, bias, target)
         need = ctx.needs_input_grad
-        ctx.grads, ctx.geometry = None, geometry
+        ctx.grads = None
         if reduction != "none" and single_pass(input, geometry, weight.shape[0]):
-            grad_x, grad_geometry = _empty_gradient(input, ctx.geometry) if need[0] else (None, None)
+            grad_x, grad_geometry = _empty_gradient(input, geometry) if need[0] else (None, None)
             grad_weight = torch.empty_like(weight) if need[1] else None
             grad_bias = torch.empty_like(bias) if bias is not None and need[2] else None
             loss, saved = xent_step_(input, geometry, weight, bias, target, ignore_index, reduction, grad_x, grad_geometry, grad_weight, grad_bias)
@@ -195,6 +203,7 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
         else:
             loss, saved = xent_forward_(input, geometry, weight, bias, target, ignore_index, reduction, True)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        ctx.layout = geometry, weight.data_ptr() % 16
         ctx.save_for_backward(input, weight, bias, target, saved)
         return loss
 
@@ -206,11 +215,14 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
             grads, ctx.grads = ctx.grads, None
             scale_([g for g in grads if g is not None], grad_loss)
             return (*grads, None, None, None)
+        # hooks on saved tensors may hand them back in another layout
+        input, weight, bias, target, geometry = _operands(input, weight, bias, target)
+        saved = _saved_for(ctx.layout, input, geometry, weight, bias, target, ctx.ignore_index, ctx.reduction, saved)
         need = ctx.needs_input_grad
-        grad_x, grad_geometry = _empty_gradient(input, ctx.geometry) if need[0] else (None, None)
+        grad_x, grad_geometry = _empty_gradient(input, geometry) if need[0] else (None, None)
         grad_weight = torch.empty_like(weight) if need[1] else None
         grad_bias = torch.empty_like(bias) if bias is not None and need[2] else None
-        xent_backward_(input, ctx.geometry, weight, bias, target, ctx.ignore_index, ctx.reduction, saved, grad_loss.contiguous(), grad_x, grad_geometry,
+        xent_backward_(input, geometry, weight, bias, target, ctx.ignore_index, ctx.reduction, saved, grad_loss.contiguous(), grad_x, grad_geometry,
                        grad_weight, grad_bias)
         return grad_x, grad_weight, grad_bias, None, None, None
 

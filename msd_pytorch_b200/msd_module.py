@@ -211,6 +211,7 @@ class MSDModuleLossFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         bias, result, fw, fb, final_weight, target, saved, *weights = ctx.saved_tensors
+        result = result.contiguous()  # hooks on saved tensors may hand it back in another layout
         if ctx.gradients is not None:
             (gradients, gfw, gfb), ctx.gradients = ctx.gradients, None
             losses.scale_([gradients, gfw, gfb], grad_loss)
