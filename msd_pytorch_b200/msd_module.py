@@ -289,6 +289,22 @@ class MSDModule(torch.nn.Module):
         c_total = self.c_in + sum(w.shape[0] for w in weights)
         if final.weight.shape[1] != c_total or input.shape[1] != self.c_in:
             raise RuntimeError("MSDModule.cross_entropy: expected %d input channels, got %d" % (self.c_in, input.shape[1]))
+        # the block's kernels take its parameters by address
+        if len(blk.dilations) != len(weights):
+            raise RuntimeError("MSDModule.cross_entropy: expected %d dilations, got %d" % (len(weights), len(blk.dilations)))
+        channels = self.c_in
+        for i, w in enumerate(weights):
+            if tuple(w.shape[1:]) != (channels, *[3] * (input.dim() - 2)):
+                raise RuntimeError("MSDModule.cross_entropy: expected weight%d of shape %s for this input, got %s" % (
+                    i, (w.shape[0], channels, *[3] * (input.dim() - 2)), tuple(w.shape)))
+            if not w.is_contiguous():
+                raise RuntimeError("MSDModule.cross_entropy: expected weight%d to be contiguous" % i)
+            channels += w.shape[0]
+        if tuple(blk.bias.shape) != (c_total - self.c_in,):
+            raise RuntimeError("MSDModule.cross_entropy: expected %d block biases, got %s" % (c_total - self.c_in, tuple(blk.bias.shape)))
+        for t in (blk.bias, *weights):
+            if t.device != input.device:
+                raise RuntimeError("MSDModule.cross_entropy: expected all tensors on %s, got one on %s" % (input.device, t.device))
         losses._check(input.detach()[:, :1], final.weight.detach()[:, :1], final.bias, target, "mean")
         if scale_in is not None and any(p.requires_grad for p in scale_in.parameters()):
             input, scale_in = scale_in(input), None
