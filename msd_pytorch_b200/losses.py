@@ -9,6 +9,7 @@ import array
 import functools
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -166,6 +167,11 @@ def scale_(tensors, factor):
     _lib.check(_lib.lib.msd_scale_tensors(spans, len(tensors), factor.data_ptr(), dev.index, _lib.stream_of(dev)))
 
 
+def _has_tangent(*tensors):
+    """Whether one of the tensors carries a forward-mode derivative."""
+    return fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _operands(input, weight, bias, target):
     """The arguments as the library takes them, and the features' geometry."""
     geometry = _features(input)
@@ -243,7 +249,8 @@ def linear_cross_entropy(input, weight, bias, target, ignore_index=-100, reducti
     NaN; a target that names no label makes the loss and the gradients that its token reaches NaN
     instead of ending the process."""
     _check(input, weight, bias, target, reduction)
-    if not (torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))):
+    wanted = torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    if not wanted and not _has_tangent(input, weight, bias):  # a tangent goes to autograd, which refuses it
         input, weight, bias, target, geometry = _operands(input, weight, bias, target)
         return xent_forward_(input, geometry, weight, bias, target, int(ignore_index), reduction, False)[0]
     return LinearCrossEntropyFunction.apply(input, weight, bias, target, int(ignore_index), reduction)
