@@ -186,19 +186,19 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ 
 }
 
 // The reduced loss, and behind the log-sum-exps the factor of the reduction.
-__device__ __forceinline__ void finish_loss(double total, int64_t count, int reduction, int64_t T_, float *loss, float *stats) {
+__device__ __forceinline__ void finish_loss(double total, int64_t count, int reduction, float *loss, const Stats &stats) {
     if (reduction == MSD_REDUCE_MEAN) loss[0] = (float)(total / (double)count);
     if (reduction == MSD_REDUCE_SUM) loss[0] = (float)total;
-    if (stats) stats[T_] = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
+    if (stats.lse) *stats.factor = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
 }
 
 // ---- forward: joining the tiles, reducing the losses ---------------------------------------------
-// Joins the (maximum, sum) pairs of all label tiles: stats[t] = lse in units of log2, losses[t];
+// Joins the (maximum, sum) pairs of all label tiles: statistics and loss of every token;
 // per block the sum of the losses and the number of tokens that count.  TX tokens x 256 / TX lanes.  A
 // block that is the only one finishes the loss too.
 template <int TX>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const float2 *part, const float *zy, const int64_t *target, int64_t ignore, int64_t T_, int64_t O,
-                                                           int slots, float *stats, float *losses, double *block_sum, int64_t *block_count, int reduction,
+                                                           int slots, const Stats stats, float *losses, double *block_sum, int64_t *block_count, int reduction,
                                                            float *loss) {
     constexpr int LANES = kThreads / TX;
     __shared__ float2 red[LANES][TX + 1];
@@ -231,14 +231,14 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const float2 *part, c
         }
         if (w == 0 && t < T_) {
             for (int i = 1; i < 8; ++i) join(m, s, red[i][x]);
-            const float lse = m + log2f(s);
+            const float log_s = log2f(s);
             const int64_t y = target[t];
             float loss = 0.f;
             if (y != ignore) {
-                loss = y >= 0 && y < O ? (lse - zy[t]) * kLn2 : CUDART_NAN_F;  // NaN: a target that names no label
+                loss = y >= 0 && y < O ? ((m - zy[t]) + log_s) * kLn2 : CUDART_NAN_F;  // NaN: a target that names no label
                 ++count;
             }
-            if (stats) stats[t] = lse;
+            if (stats.lse) stats.write(t, m, log_s);
             if (losses) losses[t] = loss;
             total += loss;
         }
@@ -248,13 +248,13 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const float2 *part, c
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < TX; ++i) total += ssum[i], count += scount[i];
-        if (gridDim.x == 1 && loss) finish_loss(total, count, reduction, T_, loss, stats);
+        if (gridDim.x == 1 && loss) finish_loss(total, count, reduction, loss, stats);
         else block_sum[blockIdx.x] = total, block_count[blockIdx.x] = count;
     }
 }
 
-__global__ void __launch_bounds__(kThreads) finish_kernel(const double *block_sum, const int64_t *block_count, int blocks, int reduction, int64_t T_, float *loss,
-                                                          float *stats) {
+__global__ void __launch_bounds__(kThreads) finish_kernel(const double *block_sum, const int64_t *block_count, int blocks, int reduction, float *loss,
+                                                          const Stats stats) {
     __shared__ double ssum[kThreads];
     __shared__ int64_t scount[kThreads];
     double total = 0;
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const double *block_su
     }
     if (threadIdx.x) return;
     total = ssum[0], count = scount[0];
-    finish_loss(total, count, reduction, T_, loss, stats);
+    finish_loss(total, count, reduction, loss, stats);
 }
 
 // ---- backward: the factor in front of the gradients -----------------------------------------------
@@ -422,7 +422,7 @@ static Operands carve_operands(const Plan &q, Carver *c) {
 // What the forward call leaves to the backward call: log-sum-exps and the reduction's factor, and,
 // unless they are large, the packed operands.
 constexpr size_t kKeptBytes = 256u << 20;
-static size_t stats_bytes(const Plan &q) { return pad256((size_t)(q.T + 1) * sizeof(float)); }
+static size_t stats_bytes(const Plan &q) { return Stats::bytes(q.T); }
 static bool keeps_operands(const Plan &q) {
     Carver c(nullptr);
     carve_operands(q, &c);
@@ -627,7 +627,7 @@ static int few_forward(const Problem &p, float *loss, float *saved, float2 *part
     else rc = launch_few<__half>(f, blocks, s);
     if (rc) return rc;
     count_launch(true);
-    few_finish_kernel<<<1, 32 * kFewTokens, 0, s>>>(part, zy, p.target, p.ignore_index, f.T, p.labels, blocks, p.reduction, loss, saved);
+    few_finish_kernel<<<1, 32 * kFewTokens, 0, s>>>(part, zy, p.target, p.ignore_index, f.T, p.labels, blocks, p.reduction, loss, Stats::of(saved, f.T));
     return launched();
 }
 
@@ -644,6 +644,7 @@ int forward(const Problem &p, float *loss, float *saved, void *ws, size_t wsb, i
         op = carve_operands(q, &k);
     }
     const int sms = fast::sm_count(device), pairs = pair_count(sms);
+    const Stats stats = Stats::of(saved, q.T);
     int64_t blocks = 0;
     bool alone = false;
     for (int64_t t0 = 0; t0 < q.T; t0 += q.chunk) {
@@ -661,13 +662,13 @@ int forward(const Problem &p, float *loss, float *saved, void *ws, size_t wsb, i
         const int tx = !alone && n <= 4096 ? 4 : 32;
         const int64_t more = alone ? 1 : ceil_div(n, tx) < kCombineBlocks ? ceil_div(n, tx) : kCombineBlocks;
         auto combine = tx == 4 ? combine_kernel<4> : combine_kernel<32>;
-        combine<<<(unsigned)more, kThreads, 0, s>>>(f.part, f.zy, p.target + t0, p.ignore_index, n, q.O, slots, saved ? saved + t0 : nullptr,
+        combine<<<(unsigned)more, kThreads, 0, s>>>(f.part, f.zy, p.target + t0, p.ignore_index, n, q.O, slots, stats.at(t0),
                                                    p.reduction == MSD_REDUCE_NONE ? loss + t0 : nullptr, f.bsum + blocks, f.bcount + blocks, p.reduction, alone ? loss : nullptr);
         XENT_TRY(launched());
         blocks += more;
     }
     if (alone) return MSD_OK;
-    finish_kernel<<<1, kThreads, 0, s>>>(f.bsum, f.bcount, (int)blocks, p.reduction, q.T, loss, saved);
+    finish_kernel<<<1, kThreads, 0, s>>>(f.bsum, f.bcount, (int)blocks, p.reduction, loss, stats);
     return launched();
 }
 
@@ -715,7 +716,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     XENT_TRY(common_params(p, q, op, t0, device, &m));
     XENT_TRY(logit_product(p, q, op, T_, o0, n, pairs, &m.p[0]));
     m.label0 = (int)o0;
-    m.stats = saved + t0, m.row_factor = b.row_factor ? b.row_factor + t0 : nullptr, m.factor = factor;
+    m.stats = Stats::of(const_cast<float *>(saved), q.T).at(t0), m.row_factor = b.row_factor ? b.row_factor + t0 : nullptr, m.factor = factor;
     m.columns = db ? b.columns : nullptr;
     m.g = b.g, m.g_width = gw, m.g_piece = g_piece;
     // |G| <= 2 in units of the factor: float16 holds it times 2^14, down to 2^-38
@@ -790,7 +791,7 @@ int backward(const Problem &p, const float *saved, const float *grad_loss, const
     if (!kept) {
         if (wsb < c.used + k.used) MSD_FAIL(MSD_ERR_WORKSPACE, "linear cross entropy backward: workspace of %zu bytes needed, %zu given", c.used + k.used, wsb);
     }
-    Factor factor{grad_loss, saved + q.T};
+    Factor factor{grad_loss, Stats::of(const_cast<float *>(saved), q.T).factor};
     if (b.row_factor) {
         const int64_t row_blocks = ceil_div(q.T, 4 * kThreads) < sms * 8 ? ceil_div(q.T, 4 * kThreads) : sms * 8;
         MSD_CUDA_TRY(cudaMemsetAsync(b.words, 0, 8, s));

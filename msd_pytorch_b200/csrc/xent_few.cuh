@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const FewParams p) 
                 float z = acc[r][t];
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
-                z = (z + b) * kLog2e;
+                // rounded as the products' epilogues round it: the backward pass goes through those
+                z = sizeof(T) == 4 ? __fadd_rn(__fmul_rn(z, kLog2e), b * kLog2e) : fmaf(z, kLog2e, b * kLog2e);
                 if (lane == 0 && t < p.T && o0 + r == y[t]) p.zy[t] = z;
                 const float up = fmaxf(top[t], z), base = up == -CUDART_INF_F ? 0.f : up;
                 sum[t] = sum[t] * exp2f(top[t] - base) + exp2f(z - base);  // a NaN logit makes the sum NaN
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const FewParams p) 
 
 // Joins the blocks and reduces the losses: one warp per token.
 __global__ void __launch_bounds__(32 * kFewTokens) few_finish_kernel(const float2 *part, const float *zy, const int64_t *target, int64_t ignore, int T_, int64_t O,
-                                                                    int blocks, int reduction, float *loss, float *saved) {
+                                                                    int blocks, int reduction, float *loss, const Stats saved) {
     __shared__ float losses[kFewTokens];
     const int t = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (t < T_) {
@@ -155,10 +156,10 @@ __global__ void __launch_bounds__(32 * kFewTokens) few_finish_kernel(const float
             join(m2, s2);
         }
         if (lane == 0) {
-            const float lse = m + log2f(s);
+            const float log_s = log2f(s);
             const int64_t y = target[t];
-            losses[t] = y == ignore ? 0.f : y >= 0 && y < O ? (lse - zy[t]) * kLn2 : CUDART_NAN_F;  // NaN: a target that names no label
-            if (saved) saved[t] = lse;
+            losses[t] = y == ignore ? 0.f : y >= 0 && y < O ? ((m - zy[t]) + log_s) * kLn2 : CUDART_NAN_F;  // NaN: a target that names no label
+            if (saved.lse) saved.write(t, m, log_s);
             if (reduction == MSD_REDUCE_NONE) loss[t] = losses[t];
         }
     }
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(32 * kFewTokens) few_finish_kernel(const float
     for (int i = 0; i < T_; ++i) total += losses[i], count += target[i] != ignore;
     if (reduction == MSD_REDUCE_MEAN) loss[0] = (float)(total / (double)count);
     if (reduction == MSD_REDUCE_SUM) loss[0] = (float)total;
-    if (saved) saved[T_] = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
+    if (saved.lse) *saved.factor = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
 }
 
 template <typename T, int N>

@@ -91,7 +91,7 @@ struct MmaParams {
     int group_m;         // rasterisation: this many row tiles pass before the next column tile
     float2 *part;        // kLse: [2 tiles_n][tokens] (maximum, sum) in units of log2
     float *zy;           // kLse: log2-scaled logit of the target
-    const float *stats;  // kGrad, kBack: log2-scaled lse per token, then the reduction's factor
+    Stats stats;  // kGrad: of the tokens
     const float *row_factor;  // kGrad: per token, or null: 1
     void *g;             // kGrad: [piece][tokens][g_width] 16-bit
     int64_t g_width, g_piece;
@@ -327,10 +327,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
             // read while the products run
             const bool in = row < q.M;
             int64_t y = p.ignore;
-            float lse = 0.f, upstream = 1.f;
+            float lse = 0.f, rest = 0.f, upstream = 1.f;
             if (USE != kBack && in) y = p.target[row];
             if (USE == kGrad && in) {
-                lse = p.stats[row];
+                p.stats.read(row, lse, rest);
                 if (p.row_factor) upstream = p.row_factor[row];
             }
             if (P == 2) {
@@ -445,12 +445,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float a = __uint_as_float(r[j + i]);
-                            v[j + i] = exp2_fast((P == 2 ? fmaf(a * f1, f2, bb[i]) : fmaf(a, kLog2e, bb[i])) - lse);
+                            v[j + i] = (P == 2 ? fmaf(a * f1, f2, bb[i]) : fmaf(a, kLog2e, bb[i])) - lse - rest;
                         }
                     }
-                    if (__any_sync(0xffffffffu, hit >= c && hit < c + 32)) {
+                    float d = 0.f;  // p - 1 of the target: exact where p is close to 1
+                    const bool any = __any_sync(0xffffffffu, hit >= c && hit < c + 32);
+                    if (any) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] -= hit == c + j ? 1.f : 0.f;
+                        for (int j = 0; j < 32; ++j) d = hit == c + j ? v[j] : d;
+                        d = expm1f(d * kLn2);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j]);
+                    if (any) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = hit == c + j ? d : v[j];
                     }
                     // columns past the last label and ignored tokens are exact zeros whatever the logits hold
 #pragma unroll

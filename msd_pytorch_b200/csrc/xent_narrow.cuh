@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(32 * kWarps, OP == 8 || OP == 12 ? 2 : 3) narr
             }
             float loss = 0.f;
             if (y[j] != p.ignore) {
-                loss = hit >= 0 ? (base + __log2f(s) - chosen) * kLn2 : CUDART_NAN_F;  // no label left: -infinity
+                loss = hit >= 0 ? ((base - chosen) + log2f(s)) * kLn2 : CUDART_NAN_F;  // no label left: infinity - infinity
                 ++count;
             }
             if (p.losses && in[j]) p.losses[n * p.V + v0 + (ALIGNED ? K * lane + j : lane + 32 * j)] = loss;
@@ -454,11 +454,10 @@ __global__ void __launch_bounds__(32 * kWarps, OP > 8 ? 1 : 2) narrow_kernel(con
             }
 #pragma unroll
             for (int q = VW; q < 32; q <<= 1) s += __shfl_xor_sync(0xffffffffu, s, q);
-            const float lse = base + __log2f(s);  // no label left: -infinity
             if (counts) {
                 // the lane with the target's logit adds the loss
                 if ((hit >= 0 && hit < OL) || (y < 0 && part == 0)) {
-                    total += y < 0 ? CUDART_NAN_F : (lse - chosen) * kLn2;
+                    total += y < 0 ? CUDART_NAN_F : ((base - chosen) + log2f(s)) * kLn2;  // no label left: infinity - infinity
                     ++count;
                 }
             }
