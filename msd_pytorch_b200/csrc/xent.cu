@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const float2 *part, c
     const int x = threadIdx.x % TX, w = threadIdx.x / TX;
     const auto join = [](float &m, float &s, const float2 &v) {
         const float up = fmaxf(m, v.x), base = up == -CUDART_INF_F ? 0.f : up;
-        s = s * exp2f(m - base) + v.y * exp2f(v.x - base);
+        s = s * exp2f((m - base) * kLog2e) + v.y * exp2f((v.x - base) * kLog2e);
         m = up;
     };
     for (int64_t t0 = blockIdx.x * (int64_t)TX; t0 < T_; t0 += gridDim.x * (int64_t)TX) {
@@ -231,11 +231,11 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const float2 *part, c
         }
         if (w == 0 && t < T_) {
             for (int i = 1; i < 8; ++i) join(m, s, red[i][x]);
-            const float log_s = log2f(s);
+            const float log_s = logf(s);
             const int64_t y = target[t];
             float loss = 0.f;
             if (y != ignore) {
-                loss = y >= 0 && y < O ? ((m - zy[t]) + log_s) * kLn2 : CUDART_NAN_F;  // NaN: a target that names no label
+                loss = y >= 0 && y < O ? (m - zy[t]) + log_s : CUDART_NAN_F;  // NaN: a target that names no label
                 ++count;
             }
             if (stats.lse) stats.write(t, m, log_s);

@@ -13,13 +13,15 @@
 // loss and 1 - p are as small as log s while m is of the logits' size: lse rounded to a float would leave
 // nothing of them (two logits near 100 and 11 apart: 27 % off).  So the target's logit is taken off m before
 // log s is added, and backward gets lse in 48 bits: its float, and what that leaves in 24 bits.
+// Logits are multiplied by log2(e) (the exponential's base is 2) once the maximum is off: a mask of the
+// type's lowest value would leave the range.
 #pragma once
 #include "common.cuh"
 
 namespace msd {
 namespace xent {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;  // logits are held in units of log 2
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct Features {  // x or dx: element (n, c, v) at data[n*sn + c*sc + v*sv]; token = n*V + v
     void *p;
@@ -28,11 +30,11 @@ struct Features {  // x or dx: element (n, c, v) at data[n*sn + c*sc + v*sv]; to
     int64_t tokens() const { return N * V; }
 };
 
-// log-sum-exps of T tokens, in units of log2, and the factor of the reduction, in one buffer.
+// log-sum-exps of T tokens and the factor of the reduction, in one buffer.
 struct Stats {
     float *lse, *factor;
     uint16_t *low;  // the rest in units of 2^-24 of lse's last place (which counts as 64 at most: the rest of
-    int8_t *high;   // m + log s is never more than log s, and log2 s <= 31): 16 bits and 8 bits of an integer
+    int8_t *high;   // m + log s is never more than log s <= 22): 16 bits and 8 bits of an integer
     static __host__ __device__ size_t lse_bytes(int64_t T) { return ((size_t)(T + 1) * sizeof(float) + 255) / 256 * 256; }
     static size_t bytes(int64_t T) { return lse_bytes(T) + ((size_t)T * 3 + 255) / 256 * 256; }
     static __host__ __device__ Stats of(void *base, int64_t T) {

@@ -108,11 +108,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const FewParams p) 
                 float z = acc[r][t];
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
-                // rounded as the products' epilogues round it: the backward pass goes through those
-                z = sizeof(T) == 4 ? __fadd_rn(__fmul_rn(z, kLog2e), b * kLog2e) : fmaf(z, kLog2e, b * kLog2e);
+                z += b;
                 if (lane == 0 && t < p.T && o0 + r == y[t]) p.zy[t] = z;
                 const float up = fmaxf(top[t], z), base = up == -CUDART_INF_F ? 0.f : up;
-                sum[t] = sum[t] * exp2f(top[t] - base) + exp2f(z - base);  // a NaN logit makes the sum NaN
+                sum[t] = sum[t] * exp2f((top[t] - base) * kLog2e) + exp2f((z - base) * kLog2e);  // a NaN logit makes the sum NaN
                 top[t] = up;
             }
         }
@@ -126,7 +125,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const FewParams p) 
         for (int i = 0; i < kFewWarps; ++i) {
             const float2 v = red[i][threadIdx.x];
             const float up = fmaxf(m, v.x), base = up == -CUDART_INF_F ? 0.f : up;
-            s = s * exp2f(m - base) + v.y * exp2f(v.x - base);
+            s = s * exp2f((m - base) * kLog2e) + v.y * exp2f((v.x - base) * kLog2e);
             m = up;
         }
         p.part[(int64_t)blockIdx.x * p.T + threadIdx.x] = make_float2(m, s);
@@ -142,7 +141,7 @@ __global__ void __launch_bounds__(32 * kFewTokens) few_finish_kernel(const float
         float m = -CUDART_INF_F, s = 0.f;
         const auto join = [&](float m2, float s2) {
             const float up = fmaxf(m, m2), base = up == -CUDART_INF_F ? 0.f : up;
-            s = s * exp2f(m - base) + s2 * exp2f(m2 - base);
+            s = s * exp2f((m - base) * kLog2e) + s2 * exp2f((m2 - base) * kLog2e);
             m = up;
         };
 #pragma unroll 4
@@ -156,9 +155,9 @@ __global__ void __launch_bounds__(32 * kFewTokens) few_finish_kernel(const float
             join(m2, s2);
         }
         if (lane == 0) {
-            const float log_s = log2f(s);
+            const float log_s = logf(s);
             const int64_t y = target[t];
-            losses[t] = y == ignore ? 0.f : y >= 0 && y < O ? ((m - zy[t]) + log_s) * kLn2 : CUDART_NAN_F;  // NaN: a target that names no label
+            losses[t] = y == ignore ? 0.f : y >= 0 && y < O ? (m - zy[t]) + log_s : CUDART_NAN_F;  // NaN: a target that names no label
             if (saved.lse) saved.write(t, m, log_s);
             if (reduction == MSD_REDUCE_NONE) loss[t] = losses[t];
         }

@@ -89,8 +89,8 @@ struct MmaParams {
     int64_t ignore;
     int labels, label0;  // kGrad: this piece covers labels [label0, label0 + p[0].N)
     int group_m;         // rasterisation: this many row tiles pass before the next column tile
-    float2 *part;        // kLse: [2 tiles_n][tokens] (maximum, sum) in units of log2
-    float *zy;           // kLse: log2-scaled logit of the target
+    float2 *part;        // kLse: [2 tiles_n][tokens] (maximum, sum of exp)
+    float *zy;           // kLse: logit of the target
     Stats stats;  // kGrad: of the tokens
     const float *row_factor;  // kGrad: per token, or null: 1
     void *g;             // kGrad: [piece][tokens][g_width] 16-bit
@@ -358,11 +358,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
             }
             const uint32_t t0 = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
             if (USE != kBack && it.n != biases_of) {
-                // this half's biases in units of log2; labels past the end count as -infinity
+                // this half's biases; labels past the end count as -infinity
                 biases_of = it.n, parity ^= 1;
                 const int i = threadIdx.x - 128 - half * 128, o = p.label0 + col0 + i;
                 bias_s[parity * kTileN + half * (kTileN / 2) + i] =
-                    i < cols && o < p.labels ? (p.bias ? load_float(p.bias, p.bias_type, o) * kLog2e : 0.f) : -CUDART_INF_F;
+                    i < cols && o < p.labels ? (p.bias ? load_float(p.bias, p.bias_type, o) : 0.f) : -CUDART_INF_F;
                 named_barrier(1 + half, 128);
             }
             const float *bias_h = bias_s + parity * kTileN + half * (kTileN / 2);
@@ -373,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 float top = -CUDART_INF_F, sum = 0.f;
                 const bool live = in;
                 const int hit = live && y >= col0 && y < col0 + cols ? (int)(y - col0) : -1;
-                const float f1 = power2(-ex) * kLog2e, f2 = power2(-ew);
+                const float f1 = power2(-ex), f2 = power2(-ew);
 #pragma unroll(P == 2 ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
@@ -393,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float v = __uint_as_float(r[j + i]);
-                            z[j + i] = P == 2 ? fmaf(v * f1, f2, bb[i]) : fmaf(v, kLog2e, bb[i]);
+                            z[j + i] = P == 2 ? fmaf(v * f1, f2, bb[i]) : v + bb[i];
                         }
                     }
                     if (c + 32 > cols) {  // columns that no product wrote
@@ -412,8 +412,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     const float base = up == -CUDART_INF_F ? 0.f : up;
                     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast(z[j] - base);  // a NaN logit makes the sum NaN
-                    sum = sum * exp2_fast(top - base) + ((s[0] + s[1]) + (s[2] + s[3]));
+                    for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast((z[j] - base) * kLog2e);  // a NaN logit makes the sum NaN
+                    sum = sum * exp2_fast((top - base) * kLog2e) + ((s[0] + s[1]) + (s[2] + s[3]));
                     top = up;
                 }
                 if (live && !*abort_flag) p.part[(int64_t)(2 * it.n + half) * q.M + row] = make_float2(top, sum);
@@ -422,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 float g = counts ? upstream * p.g_scale : 0.f;
                 if (counts && (y < 0 || y >= p.labels)) g = CUDART_NAN_F;
                 const int hit = y >= p.label0 + col0 && y < p.label0 + col0 + cols ? (int)(y - p.label0 - col0) : -1;
-                const float f1 = power2(-ex) * kLog2e, f2 = power2(-ew);
+                const float f1 = power2(-ex), f2 = power2(-ew);
                 const int stored = (int)min((int64_t)width, p.g_width - col0);
                 const bool ok = !*abort_flag;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
@@ -445,7 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float a = __uint_as_float(r[j + i]);
-                            v[j + i] = (P == 2 ? fmaf(a * f1, f2, bb[i]) : fmaf(a, kLog2e, bb[i])) - lse - rest;
+                            v[j + i] = (P == 2 ? fmaf(a * f1, f2, bb[i]) : a + bb[i]) - lse - rest;
                         }
                     }
                     float d = 0.f;  // p - 1 of the target: exact where p is close to 1
@@ -453,10 +453,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     if (any) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) d = hit == c + j ? v[j] : d;
-                        d = expm1f(d * kLn2);
+                        d = expm1f(d);
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j]);
+                    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j] * kLog2e);
                     if (any) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = hit == c + j ? d : v[j];

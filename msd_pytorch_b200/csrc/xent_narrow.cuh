@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(32 * kWarps, OP == 8 || OP == 12 ? 2 : 3) narr
             for (int o = 0; o < OP; ++o) {
                 float a, b;
                 unpair(z2[j / 2][o], a, b);
-                z[o] = ((j & 1 ? b : a) + bs[o]) * kLog2e;
+                z[o] = (j & 1 ? b : a) + bs[o];
                 top = fmaxf(top, z[o]);
             }
             const float base = top == -CUDART_INF_F ? 0.f : top;
@@ -233,12 +233,12 @@ __global__ void __launch_bounds__(32 * kWarps, OP == 8 || OP == 12 ? 2 : 3) narr
             float s = 0.f, chosen = 0.f;
 #pragma unroll
             for (int o = 0; o < OP; ++o) {
-                s += exp2_narrow(z[o] - base);  // NaN logits: a NaN sum
+                s += exp2_narrow((z[o] - base) * kLog2e);  // NaN logits: a NaN sum
                 if (o == hit) chosen = z[o];
             }
             float loss = 0.f;
             if (y[j] != p.ignore) {
-                loss = hit >= 0 ? ((base - chosen) + log2f(s)) * kLn2 : CUDART_NAN_F;  // no label left: infinity - infinity
+                loss = hit >= 0 ? (base - chosen) + logf(s) : CUDART_NAN_F;  // no label left: infinity - infinity
                 ++count;
             }
             if (p.losses && in[j]) p.losses[n * p.V + v0 + (ALIGNED ? K * lane + j : lane + 32 * j)] = loss;
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(32 * kWarps, OP > 8 ? 1 : 2) narrow_kernel(con
             float top = -CUDART_INF_F;
 #pragma unroll
             for (int o = 0; o < OL; ++o) {
-                z[o] = (z[o] + bs[part * OL + o]) * kLog2e;
+                z[o] += bs[part * OL + o];
                 top = fmaxf(top, z[o]);
             }
 #pragma unroll
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(32 * kWarps, OP > 8 ? 1 : 2) narrow_kernel(con
             const int hit = y - part * OL;
 #pragma unroll
             for (int o = 0; o < OL; ++o) {
-                e[o] = exp2_narrow(z[o] - base);  // NaN logits: a NaN sum
+                e[o] = exp2_narrow((z[o] - base) * kLog2e);  // NaN logits: a NaN sum
                 s += e[o];
                 if (o == hit) chosen = z[o];
             }
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(32 * kWarps, OP > 8 ? 1 : 2) narrow_kernel(con
             if (counts) {
                 // the lane with the target's logit adds the loss
                 if ((hit >= 0 && hit < OL) || (y < 0 && part == 0)) {
-                    total += y < 0 ? CUDART_NAN_F : ((base - chosen) + log2f(s)) * kLn2;  // no label left: infinity - infinity
+                    total += y < 0 ? CUDART_NAN_F : (base - chosen) + logf(s);  // no label left: infinity - infinity
                     ++count;
                 }
             }
