@@ -39,61 +39,9 @@ struct Matrix {  // row r, column c at p[(t / V) sn + (t % V) sv + c sc], t = ro
     __device__ __forceinline__ bool dropped(int64_t r) const { return target && target[row0 + r] == ignore; }
 };
 
-constexpr int kMaxBlocks = 1184;  // blocks of max_kernel per matrix, at most
-constexpr int kMaxStretch = 32;   // columns that a thread of it takes at a time
-
-// Largest finite magnitude of x and of W as the bits of a float: one value per block (a maximum does
-// not depend on its order).  Blocks [0, blocks_x) take x, the others W.
-__global__ void __launch_bounds__(kThreads) max_kernel(const Matrix x, const Matrix w, int blocks_x, uint32_t *block_max) {
-    __shared__ uint32_t red[kThreads / 32];
-    const bool first = (int)blockIdx.x < blocks_x;
-    const Matrix &a = first ? x : w;
-    const int block = first ? blockIdx.x : blockIdx.x - blocks_x, blocks = first ? blocks_x : gridDim.x - blocks_x;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t m = 0;
-    const auto take = [&](float v) {
-        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-        m = b < 0x7f800000u ? max(m, b) : m;
-    };
-    if (a.sc == 1) {  // a warp per row
-        const bool vec = a.cols % 4 == 0 && ((uintptr_t)a.p & 15) == 0 && a.sv % 4 == 0 && a.sn % 4 == 0;
-        for (int64_t r = (int64_t)block * (kThreads / 32) + warp; r < a.rows; r += (int64_t)blocks * (kThreads / 32)) {
-            if (a.dropped(r)) continue;
-            const float *row = (const float *)a.p + a.row_start(r);
-            if (vec) {
-#pragma unroll 4
-                for (int64_t c = lane * 4; c < a.cols; c += 128) {
-                    const float4 v = *reinterpret_cast<const float4 *>(row + c);
-                    take(v.x), take(v.y), take(v.z), take(v.w);
-                }
-            } else {
-#pragma unroll 8
-                for (int64_t c = lane; c < a.cols; c += 32) take(row[c]);
-            }
-        }
-    } else {  // a thread per row (neighbours lie side by side in a column) and stretch of columns
-        const int64_t stretches = (a.cols + kMaxStretch - 1) / kMaxStretch, groups = (a.rows + kThreads - 1) / kThreads;
-        for (int64_t g = block; g < groups * stretches; g += blocks) {
-            const int64_t r = g / stretches * kThreads + threadIdx.x, c0 = g % stretches * kMaxStretch, c1 = min(a.cols, c0 + kMaxStretch);
-            if (r >= a.rows || a.dropped(r)) continue;
-            const float *row = (const float *)a.p + a.row_start(r);
-#pragma unroll 8
-            for (int64_t c = c0; c < c1; ++c) take(row[c * a.sc]);
-        }
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < kThreads / 32; ++i) m = max(m, red[i]);
-        block_max[first ? block : kMaxBlocks + block] = m;
-    }
-}
-
 // dst[piece][row][ld] 16-bit: an operand row by row, columns past the last as zeros.  Blocks of 64
 // rows x 64 columns pass through shared memory, read along whichever axis is dense.  Blocks
-// [0, blocks_x) are x's, the others W's.  Two pieces: every block finds the largest magnitudes among
-// max_kernel's, and the first of each matrix leaves it in words[] for the products' epilogues.
+// [0, blocks_x) are x's, the others W's.  Three pieces: see xent_mma.cuh.
 constexpr int kPackRows = 64, kPackCols = 64;
 struct PackParams {
     Matrix m[2];
@@ -101,19 +49,20 @@ struct PackParams {
     int64_t ld;
     int64_t blocks_x;
     int col_blocks;
-    int max_blocks[2];
-    const uint32_t *block_max;
-    uint32_t *words;
 };
+// The bfloat16 next to v; the largest one where the next would be infinity.
+__device__ __forceinline__ uint16_t top_piece(float v) {
+    const uint16_t b = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    return (b & 0x7fff) == 0x7f80 && fabsf(v) < CUDART_INF_F ? b - 1 : b;
+}
 template <typename T, int P>
 __global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ PackParams p) {
     __shared__ T tile[kPackRows][kPackCols + 1];
-    __shared__ uint32_t red[kThreads / 32];
     const int which = blockIdx.x < p.blocks_x ? 0 : 1;
     const int64_t block = blockIdx.x - (which ? p.blocks_x : 0);
     const Matrix &a = p.m[which];
     const int64_t r0 = block / p.col_blocks * kPackRows, c0 = block % p.col_blocks * kPackCols;
-    // values first: nothing waits for targets or magnitudes
+    // values first: nothing waits for targets
     if (a.sc == 1) {
         const int c = threadIdx.x % kPackCols;
         const bool in = c0 + c < a.cols;
@@ -142,19 +91,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < kPackCols / (kThreads / kPackRows); ++k) tile[r][threadIdx.x / kPackRows + k * (kThreads / kPackRows)] = drop ? T(0.f) : v[k];
     }
-    float scale = 1.f;
-    if (P == 2) {
-        uint32_t m = 0;
-        for (int i = threadIdx.x; i < p.max_blocks[which]; i += kThreads) m = max(m, p.block_max[which * kMaxBlocks + i]);
-        m = __reduce_max_sync(0xffffffffu, m);
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-        __syncthreads();
-        for (int i = 0; i < kThreads / 32; ++i) m = max(m, red[i]);
-        if (block == 0 && threadIdx.x == 0) p.words[which] = m;
-        scale = power2(scale_exponent(m));
-    } else {
-        __syncthreads();
-    }
+    __syncthreads();
     const int64_t piece = a.rows * p.ld;
     const int c = threadIdx.x % (kPackCols / 4) * 4;  // ld is a multiple of 8: four columns are all in or all out
     const int64_t col = c0 + c;
@@ -164,18 +101,19 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ 
         const int64_t row = r0 + r;
         if (row >= a.rows) break;
         uint16_t *out = p.dst[which] + row * p.ld + col;
-        if constexpr (P == 2) {
-            uint32_t hi[2], lo[2];
+        if constexpr (P == 3) {
+            uint16_t h[3][4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float v0 = (float)tile[r][c + 2 * k] * scale, v1 = (float)tile[r][c + 2 * k + 1] * scale;
-                const __half2 h = __floats2half2_rn(v0, v1);
-                const float d0 = v0 - __low2float(h), d1 = v1 - __high2float(h);  // NaN for infinities: those have no second piece
-                const __half2 l = __floats2half2_rn(fabsf(v0) < CUDART_INF_F ? d0 : 0.f, fabsf(v1) < CUDART_INF_F ? d1 : 0.f);
-                memcpy(hi + k, &h, 4), memcpy(lo + k, &l, 4);
+            for (int k = 0; k < 4; ++k) {
+                const float v = (float)tile[r][c + k];
+                h[0][k] = top_piece(v);
+                const float d = fabsf(v) < CUDART_INF_F ? v - __bfloat162float(__ushort_as_bfloat16(h[0][k])) : 0.f;  // infinities have one piece
+                const __nv_bfloat16 m = __float2bfloat16_rn(d);
+                h[1][k] = __bfloat16_as_ushort(m), h[2][k] = __bfloat16_as_ushort(__float2bfloat16_rn(d - __bfloat162float(m)));
             }
-            *reinterpret_cast<uint2 *>(out) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2 *>(out + piece) = make_uint2(lo[0], lo[1]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                *reinterpret_cast<uint2 *>(out + i * piece) = make_uint2((uint32_t)h[i][0] | ((uint32_t)h[i][1] << 16), (uint32_t)h[i][2] | ((uint32_t)h[i][3] << 16));
         } else {
             uint16_t h[4];
 #pragma unroll
@@ -358,8 +296,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
         q.sum[j] = (float)s;
         return;
     }
-    const float f1 = p.max_bits ? power2(-scale_exponent(p.max_bits[which == 0 ? 1 : 0])) : 1.f;
-    store(q.out, out_type, ((q.row0 + m) / q.V) * q.sn + ((q.row0 + m) % q.V) * q.sm + n * q.sc, (float)s * f1 * (p.factor.value() / p.g_scale));
+    store(q.out, out_type, ((q.row0 + m) / q.V) * q.sn + ((q.row0 + m) % q.V) * q.sm + n * q.sc, (float)s * (p.factor.value() / p.g_scale));
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -373,10 +310,10 @@ struct Plan {
 
 static Plan make_plan(const Problem &p) {
     Plan q;
-    q.P = p.dtype == MSD_F32 ? 2 : 1;
+    q.P = p.dtype == MSD_F32 ? 3 : 1;
     q.T = p.x.tokens(), q.C = p.x.C, q.O = p.labels;
     q.ld = round_up(q.C, 8);
-    q.pack_w = q.P == 2 || q.C % 8 || ((uintptr_t)p.weight & 15);
+    q.pack_w = q.P > 1 || q.C % 8 || ((uintptr_t)p.weight & 15);
     q.chunk = kChunkBytes / (2 * q.P * q.ld) / kTileM * kTileM;
     if (q.chunk < 16 * kTileM) q.chunk = 16 * kTileM;
     if (q.chunk > q.T) q.chunk = q.T;
@@ -406,14 +343,10 @@ struct Carver {
 
 struct Operands {
     uint16_t *x, *w;
-    uint32_t *words;  // [0], [1]: magnitudes of x and W
-    uint32_t *block_max;
 };
 
 static Operands carve_operands(const Plan &q, Carver *c) {
     Operands o;
-    o.words = c->take<uint32_t>(64);
-    o.block_max = c->take<uint32_t>(2 * kMaxBlocks);
     o.x = c->take<uint16_t>(q.P * q.chunk * q.ld);
     o.w = q.pack_w ? c->take<uint16_t>(q.P * q.O * q.ld) : nullptr;
     return o;
@@ -527,33 +460,19 @@ static int launched() {
         if (rc__) return rc__;   \
     } while (0)
 
-// Packs the tokens [t0, t0 + n) of x and, with the first of them, W where needed.  Two pieces: the first
-// call also finds the largest magnitudes, of all of x.
+// Packs the tokens [t0, t0 + n) of x and, with the first of them, W where needed.
 static int pack_operands(const Problem &p, const Plan &q, const Operands &op, int64_t t0, int64_t n, cudaStream_t s) {
     PackParams k;
-    k.m[0] = Matrix{p.x.p, q.T, q.C, p.x.V, p.x.sn, p.x.sv, p.x.sc, p.target, p.ignore_index, 0, p.x.N == 1};
+    k.m[0] = Matrix{p.x.p, n, q.C, p.x.V, p.x.sn, p.x.sv, p.x.sc, p.target, p.ignore_index, t0, p.x.N == 1};
     k.m[1] = Matrix{p.weight, q.O, q.C, q.O, 0, q.C, 1, nullptr, 0, 0, true};
     k.dst[0] = op.x, k.dst[1] = op.w;
     k.ld = q.ld;
-    k.block_max = op.block_max, k.words = op.words;
     k.col_blocks = (int)ceil_div(q.ld, kPackCols);
     const int64_t bx = ceil_div(n, kPackRows) * k.col_blocks, bw = q.pack_w && t0 == 0 ? ceil_div(q.O, kPackRows) * k.col_blocks : 0;
     if (bx + bw > 0x7fffffff) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: %lld labels times %lld channels are too many", (long long)q.O, (long long)q.C);
     k.blocks_x = bx;
-    if (q.P == 2) {
-        for (int i = 0; i < 2; ++i) {
-            const Matrix &m = k.m[i];
-            const int64_t most = m.sc == 1 ? ceil_div(m.rows, kThreads / 32) : ceil_div(m.rows, kThreads) * ceil_div(m.cols, kMaxStretch);
-            k.max_blocks[i] = (int)(most < kMaxBlocks ? most : kMaxBlocks);
-        }
-        if (t0 == 0) {
-            max_kernel<<<k.max_blocks[0] + k.max_blocks[1], kThreads, 0, s>>>(k.m[0], k.m[1], k.max_blocks[0], op.block_max);
-            XENT_TRY(launched());
-        }
-    }
-    k.m[0].rows = n, k.m[0].row0 = t0;
     const unsigned grid = (unsigned)(bx + bw);
-    if (p.dtype == MSD_F32) pack_kernel<float, 2><<<grid, kThreads, 0, s>>>(k);
+    if (p.dtype == MSD_F32) pack_kernel<float, 3><<<grid, kThreads, 0, s>>>(k);
     else if (p.dtype == MSD_BF16) pack_kernel<__nv_bfloat16, 1><<<grid, kThreads, 0, s>>>(k);
     else pack_kernel<__half, 1><<<grid, kThreads, 0, s>>>(k);
     return launched();
@@ -561,19 +480,19 @@ static int pack_operands(const Problem &p, const Plan &q, const Operands &op, in
 
 template <int USE>
 static int launch_mma(const MmaParams &m, int P, int pairs, cudaStream_t s) {
-    auto kern = P == 2 ? xent_mma_kernel<USE, 2> : xent_mma_kernel<USE, 1>;
+    auto kern = P > 1 ? xent_mma_kernel<USE, 3> : xent_mma_kernel<USE, 1>;
     const size_t smem = mma_smem_bytes(P);
-    static std::atomic<uint64_t> ready[2];  // devices whose kernel is set up, per number of pieces
+    static std::atomic<uint64_t> ready[2];  // devices whose kernel is set up, for one piece and for three
     int device = 0;
     MSD_CUDA_TRY(cudaGetDevice(&device));
-    if (device >= 64 || !(ready[P - 1].load() >> device & 1)) {
-        if (P == 2) {
+    if (device >= 64 || !(ready[P > 1].load() >> device & 1)) {
+        if (P > 1) {
             cudaFuncAttributes a;
             MSD_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
             if (a.numRegs < kRegsLaunch) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: built with %d registers per thread, %d expected", a.numRegs, kRegsLaunch);
         }
         MSD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        if (device < 64) ready[P - 1].fetch_or(1ull << device);
+        if (device < 64) ready[P > 1].fetch_or(1ull << device);
     }
     kern<<<2 * pairs, kMmaThreads, smem, s>>>(m);
     return launched();
@@ -582,8 +501,7 @@ static int launch_mma(const MmaParams &m, int P, int pairs, cudaStream_t s) {
 // What the three uses have in common.
 static int common_params(const Problem &p, const Plan &q, const Operands &op, int64_t t0, int device, MmaParams *m) {
     memset(m, 0, sizeof(*m));
-    m->bf16 = p.dtype == MSD_BF16;
-    m->max_bits = q.P == 2 ? op.words : nullptr;
+    m->bf16 = p.dtype == MSD_BF16 || q.P > 1;
     m->bias = p.bias, m->bias_type = p.dtype;
     m->target = p.target + t0, m->ignore = p.ignore_index, m->labels = (int)q.O;
     m->group_m = 64;  // 8192 rows of x: 16 MB at 1024 channels
@@ -719,8 +637,8 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     m.stats = Stats::of(const_cast<float *>(saved), q.T).at(t0), m.row_factor = b.row_factor ? b.row_factor + t0 : nullptr, m.factor = factor;
     m.columns = db ? b.columns : nullptr;
     m.g = b.g, m.g_width = gw, m.g_piece = g_piece;
-    // |G| <= 2 in units of the factor: float16 holds it times 2^14, down to 2^-38
-    m.g_scale = p.dtype == MSD_BF16 ? 1.f : 16384.f;
+    // |G| <= 2 in units of the factor: one float16 holds it times 2^14, down to 2^-38
+    m.g_scale = p.dtype == MSD_F16 ? 16384.f : 1.f;
     const int64_t tiles = (int64_t)m.p[0].tiles_m * m.p[0].tiles_n;
     XENT_TRY(launch_mma<kGrad>(m, q.P, (int)(tiles < pairs ? tiles : pairs), s));
     if (db) {

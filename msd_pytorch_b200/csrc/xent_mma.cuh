@@ -5,12 +5,13 @@
 //   kGrad   the same product again, epilogue: G = exp(z - lse) - onehot, rounded to 16 bits, stored
 //   kBack   dx = G W and dW = G^T x: two lists of tiles in one launch, longest first
 //
-// Operands are 16-bit: bfloat16 and float16 inputs as they are, float32 inputs as the sum of two
-// float16 pieces v s = hi + lo (s: a power of two that brings the tensor's largest value
-// into [2^14, 2^15)); hi carries 11 bits of the value, lo the next 11, and a product is
-// hi hi' + hi lo' + lo hi' (the dropped lo lo' is below 2^-24 of the product): float32-level
-// accuracy in three products.  Pieces below 2^-24 (2^-39 of the largest value) are lost: a
-// fixed point for values far below the tensor's largest.
+// Operands are 16-bit: bfloat16 and float16 inputs as they are, float32 inputs as the sum of three
+// bfloat16 pieces v = a + b + c of 8 bits each (round to nearest: |b| <= 2^-9 |v|, |c| <= 2^-18 |v|, and
+// 2^-27 |v| is left).  A product is a a' + (a b' + b a') + (a c' + b b' + c a'): what is dropped is below
+// 2^-25 of it, less than a float32 product's own rounding, and as the pieces have float32's range of exponents
+// this holds whatever the other values of the tensor are.  (Two float16 pieces under one power of two
+// per tensor need three products instead of six, but lose values 2^-24 below the tensor's largest step by
+// step: one token of 1e8 took 8 bits from all others.)
 //
 // The tensor core's float32 additions truncate: a sum of n of them is off by up to n 2^-23 and
 // drifts towards zero (dW over 65536 tokens: 8e-6 off; a rounding sum 2e-7).  For float32 inputs
@@ -48,7 +49,7 @@ static_assert(kRegsIssue * 128 + kRegsEpilogue * 256 <= kRegsLaunch * kMmaThread
 
 enum Use { kLse = 0, kGrad = 1, kBack = 2 };
 
-__host__ __device__ constexpr int stages_of(int pieces) { return pieces == 1 ? 6 : 3; }
+__host__ __device__ constexpr int stages_of(int pieces) { return pieces == 1 ? 6 : 2; }
 __host__ __device__ constexpr size_t mma_smem_bytes(int pieces) {
     return 1024 + (size_t)stages_of(pieces) * pieces * (kABytes + kBBytes) + 2 * kTileN * sizeof(float) + 8 * 32 * kTurn * sizeof(float) + 256;
 }
@@ -81,7 +82,6 @@ struct Factor {
 struct MmaParams {
     Product p[2];  // kLse, kGrad: [0]; kBack: [0] = dx, [1] = dW
     bool bf16;     // operand type: bfloat16, else float16
-    const uint32_t *max_bits;  // two pieces: the largest magnitudes of x and W (bits of a float); null otherwise
     // kLse, kGrad
     const void *bias;
     int bias_type;
@@ -171,10 +171,10 @@ struct Items {  // this pair's work, in order
     }
 };
 
-// Results of P pieces: float32 for two, 16 bits for one.
+// Results of P pieces: float32 for three, 16 bits for one.
 template <int P>
 __device__ __forceinline__ void store_one(void *out, bool bf16, int64_t i, float v) {
-    if (P == 2) ((float *)out)[i] = v;
+    if (P > 1) ((float *)out)[i] = v;
     else if (bf16) ((__nv_bfloat16 *)out)[i] = __float2bfloat16_rn(v);
     else ((__half *)out)[i] = __float2half_rn(v);
 }
@@ -189,6 +189,8 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float a, float b) {
 template <int USE, int P>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent_mma_kernel(const __grid_constant__ MmaParams p) {
     using namespace tma;
+    static_assert(P == 1 || P == 3, "operands as they are, or in three pieces");
+    constexpr bool WIDE = P > 1;
     constexpr int S = stages_of(P);
     constexpr int kStage = P * (kABytes + kBBytes);
     extern __shared__ unsigned char xent_smem[];
@@ -211,10 +213,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
     umma::cluster_sync();  // both CTAs' barriers exist from here on
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    // Two pieces: the epilogue warps keep 128 sums per thread.  kRegsIssue x 128 + kRegsEpilogue x 256 is
+    // Three pieces: the epilogue warps keep 128 sums per thread.  kRegsIssue x 128 + kRegsEpilogue x 256 is
     // what the block was launched with (kRegsLaunch x 384; the launcher checks the compiled kernel).
     if (warp < 4) {
-        if (P == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // The loops of both issuing warps run with all lanes (see umma::elect_one): with one lane in a
         // branch of its own the products of 64 took 1000 clocks to issue instead of the 512 they run.
         if (warp == 0) {
@@ -274,7 +276,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 // 8192 bytes, 8 k at 1024, so 16 k = 2048 bytes.
                 const uint32_t a_step = q.a_mn ? 2048 / 16 : 32 / 16, b_step = q.b_mn ? 2048 / 16 : 32 / 16;
                 for (int kb = it.k0; kb < it.k1; ++kb) {
-                    const bool first = P == 2 || kb == it.k0;
+                    const bool first = WIDE || kb == it.k0;
                     if (first) {
                         wait_parity(acc_empty + acc, acc_phase ^ 1, abort_flag, p.status, 22);
                         __syncwarp();
@@ -286,19 +288,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     umma::fence_after_sync();
                     const uint32_t a = lo0 + (uint32_t)(stage * kStage) / 16, b = a + P * kABytes / 16;
                     const int steps = min(kDepth / 16, (K - kb * kDepth + 15) / 16);
-                    const bool sum_done = P == 2 || kb + 1 == it.k1;
+                    const bool sum_done = WIDE || kb + 1 == it.k1;
                     if (umma::elect_one()) {
-                        if (P == 2) {  // the small products first
+                        // pieces whose orders add up to 2, then 1, then 0: the small products first
+#pragma unroll
+                        for (int order = P - 1; order >= 0; --order)
 #pragma unroll
                             for (int ks = 0; ks < kDepth / 16; ++ks)
-                                if (ks < steps) {
-                                    umma::mma_f16_pair(d, umma::desc_words(a + ks * a_step, hi), umma::desc_words(b + kBBytes / 16 + ks * b_step, hi), idesc, ks > 0);
-                                    umma::mma_f16_pair(d, umma::desc_words(a + kABytes / 16 + ks * a_step, hi), umma::desc_words(b + ks * b_step, hi), idesc, 1);
-                                }
-                        }
+                                if (ks < steps)
 #pragma unroll
-                        for (int ks = 0; ks < kDepth / 16; ++ks)
-                            if (ks < steps) umma::mma_f16_pair(d, umma::desc_words(a + ks * a_step, hi), umma::desc_words(b + ks * b_step, hi), idesc, P == 2 || ks > 0 || !first);
+                                    for (int i = 0; i <= order; ++i)
+                                        umma::mma_f16_pair(d, umma::desc_words(a + i * (kABytes / 16) + ks * a_step, hi),
+                                                           umma::desc_words(b + (order - i) * (kBBytes / 16) + ks * b_step, hi), idesc,
+                                                           order < P - 1 || ks > 0 || i > 0 || !first);
                         umma::commit_pair(empty + stage);
                         if (sum_done) umma::commit_pair(acc_full + acc);
                     }
@@ -310,15 +312,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
         }
         __syncwarp();
     } else {
-        if (P == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+        if (WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         const int half = (warp - 4) >> 2, quad = warp & 3;
         Items<USE> items(p);
         Item it;
         int acc = 0;
         uint32_t acc_phase = 0;
         int parity = 0, biases_of = -1;
-        float run_sums[P == 2 ? kTileN / 2 : 1];  // sums of the contraction so far
-        const int ex = P == 2 ? scale_exponent(p.max_bits[0]) : 0, ew = P == 2 ? scale_exponent(p.max_bits[1]) : 0;
+        float run_sums[WIDE ? kTileN / 2 : 1];  // sums of the contraction so far
         while (items.get(it)) {
             const Product &q = p.p[it.which];
             const int row = it.m * kTileM + (int)rank * kCtaM + quad * 32 + lane;  // token (kBack, dW: label)
@@ -333,9 +334,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 p.stats.read(row, lse, rest);
                 if (p.row_factor) upstream = p.row_factor[row];
             }
-            if (P == 2) {
+            if (WIDE) {
 #pragma unroll
-                for (int j = 0; j < kTileN / 2; ++j) run_sums[P == 2 ? j : 0] = 0.f;
+                for (int j = 0; j < kTileN / 2; ++j) run_sums[WIDE ? j : 0] = 0.f;
                 for (int kb = it.k0; kb + 1 < it.k1; ++kb) {
                     wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 25);
                     __syncwarp();
@@ -348,7 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                         umma::tmem_ld32_issue(t + c, r);
                         umma::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) run_sums[P == 2 ? c + j : 0] += __uint_as_float(r[j]);
+                        for (int j = 0; j < 32; ++j) run_sums[WIDE ? c + j : 0] += __uint_as_float(r[j]);
                     }
                     umma::fence_before_sync();
                     __syncwarp();
@@ -373,17 +374,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 float top = -CUDART_INF_F, sum = 0.f;
                 const bool live = in;
                 const int hit = live && y >= col0 && y < col0 + cols ? (int)(y - col0) : -1;
-                const float f1 = power2(-ex), f2 = power2(-ew);
-#pragma unroll(P == 2 ? 4 : 1)
+#pragma unroll(WIDE ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
                     uint32_t r[32];
                     __syncwarp();
                     umma::tmem_ld32_issue(t0 + c, r);
                     umma::tmem_ld_wait();
-                    if (P == 2) {
+                    if (WIDE) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[P == 2 ? c + j : 0]);
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[WIDE ? c + j : 0]);
                     }
                     float z[32], m = -CUDART_INF_F;
 #pragma unroll
@@ -393,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float v = __uint_as_float(r[j + i]);
-                            z[j + i] = P == 2 ? fmaf(v * f1, f2, bb[i]) : v + bb[i];
+                            z[j + i] = v + bb[i];
                         }
                     }
                     if (c + 32 > cols) {  // columns that no product wrote
@@ -422,20 +422,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 float g = counts ? upstream * p.g_scale : 0.f;
                 if (counts && (y < 0 || y >= p.labels)) g = CUDART_NAN_F;
                 const int hit = y >= p.label0 + col0 && y < p.label0 + col0 + cols ? (int)(y - p.label0 - col0) : -1;
-                const float f1 = power2(-ex), f2 = power2(-ew);
                 const int stored = (int)min((int64_t)width, p.g_width - col0);
                 const bool ok = !*abort_flag;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
-#pragma unroll(P == 2 ? 4 : 1)
+#pragma unroll(WIDE ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= stored) continue;
                     uint32_t r[32];
                     __syncwarp();
                     umma::tmem_ld32_issue(t0 + c, r);
                     umma::tmem_ld_wait();
-                    if (P == 2) {
+                    if (WIDE) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[P == 2 ? c + j : 0]);
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[WIDE ? c + j : 0]);
                     }
                     float v[32];
 #pragma unroll
@@ -445,7 +444,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float a = __uint_as_float(r[j + i]);
-                            v[j + i] = (P == 2 ? fmaf(a * f1, f2, bb[i]) : a + bb[i]) - lse - rest;
+                            v[j + i] = (a + bb[i]) - lse - rest;
                         }
                     }
                     float d = 0.f;  // p - 1 of the target: exact where p is close to 1
@@ -475,9 +474,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                             if (P == 1) {
                                 w[j] = pack16(p.bf16, v[2 * j], v[2 * j + 1]);
                             } else {
-                                __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                                if (piece == 1) h = __floats2half2_rn(v[2 * j] - __low2float(h), v[2 * j + 1] - __high2float(h));
-                                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                                float v0 = v[2 * j], v1 = v[2 * j + 1];
+#pragma unroll
+                                for (int i = 0; i < piece; ++i) {
+                                    const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+                                    v0 -= __low2float(h), v1 -= __high2float(h);
+                                }
+                                w[j] = pack16(true, v0, v1);
                             }
                         }
                         __syncwarp();
@@ -508,13 +511,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 }
             } else {
                 const bool ok = !*abort_flag, live = row < q.M && ok;
-                const float f1 = power2(P == 2 ? -(it.which == 0 ? ew : ex) : 0), f2 = p.factor.value() / p.g_scale;
+                const float f = p.factor.value() / p.g_scale;
                 const bool split = q.splits > 1, done = !split && q.last;
                 float *run = split ? q.part + ((int64_t)it.split * q.M + row) * q.ld : q.sum + (int64_t)row * q.ld;
                 const bool add = !split && q.add;
                 const int64_t at = q.linear ? (q.row0 + row) * q.sm : ((q.row0 + row) / q.V) * q.sn + ((q.row0 + row) % q.V) * q.sm;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
-#pragma unroll(P == 2 ? 4 : 1)
+#pragma unroll(WIDE ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
                     uint32_t r[32];
@@ -523,7 +526,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     umma::tmem_ld_wait();
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + (P == 2 ? run_sums[P == 2 ? c + j : 0] : 0.f);
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + (WIDE ? run_sums[WIDE ? c + j : 0] : 0.f);
                     const int col = col0 + c;
                     if (add && live) {
 #pragma unroll
@@ -542,14 +545,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                         continue;
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = v[j] * f1 * f2;
+                    for (int j = 0; j < 32; ++j) v[j] *= f;
                     if (q.vec) {  // 16-byte pieces, 64 bytes of a row together: turned as in kGrad
 #pragma unroll
-                        for (int h = 0; h < P; ++h) {
+                        for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
                             __syncwarp();
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                if (P == 2) {
+                                if (WIDE) {
                                     const float *f = v + 16 * h + 4 * j;
                                     *reinterpret_cast<float4 *>(turn + lane * kTurn + 4 * j) = make_float4(f[0], f[1], f[2], f[3]);
                                 } else {
@@ -559,12 +562,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                                 }
                             }
                             __syncwarp();
-                            const int j = lane & 3, piece = P == 2 ? 16 * h + 4 * j : 8 * j;  // first of the lane's columns
+                            const int j = lane & 3, piece = WIDE ? 16 * h + 4 * j : 8 * j;  // first of the lane's columns
 #pragma unroll
                             for (int i = lane >> 2; i < 32; i += 8) {
                                 const int64_t there = __shfl_sync(0xffffffffu, at, i) + col + piece;
                                 if (ok && row - lane + i < q.M && c + piece < cols)
-                                    *reinterpret_cast<uint4 *>((char *)q.out + there * (P == 2 ? 4 : 2)) = *reinterpret_cast<const uint4 *>(turn + i * kTurn + 4 * j);
+                                    *reinterpret_cast<uint4 *>((char *)q.out + there * (WIDE ? 4 : 2)) = *reinterpret_cast<const uint4 *>(turn + i * kTurn + 4 * j);
                             }
                         }
                     } else if (q.sc != 1) {  // neighbouring tokens lie side by side: each column is a dense store of the warp
