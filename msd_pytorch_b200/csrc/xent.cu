@@ -209,27 +209,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const double *block_su
     finish_loss(total, count, reduction, loss, stats);
 }
 
-// ---- backward: the factor in front of the gradients -----------------------------------------------
-// The largest finite |grad_loss| of the tokens that count (reduction none).
-__global__ void __launch_bounds__(kThreads) upstream_max_kernel(const float *grad_loss, const int64_t *target, int64_t ignore, int64_t T_, uint32_t *out) {
-    uint32_t m = 0;
-    for (int64_t t = blockIdx.x * (int64_t)kThreads + threadIdx.x; t < T_; t += (int64_t)gridDim.x * kThreads) {
-        const float v = fabsf(grad_loss[t]);
-        if (target[t] != ignore && v < CUDART_INF_F) m = max(m, __float_as_uint(v));
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
-}
-
-// reduction none: row_factor[t] = grad_loss[t] / f with f the power of two that brings the largest
-// into [1, 2), factor = f.
-__global__ void __launch_bounds__(kThreads) factor_kernel(const float *grad_loss, int64_t T_, const uint32_t *max_bits, float *row_factor, float *factor) {
-    const int e = 14 - scale_exponent(*max_bits);
-    const float up = *max_bits ? power2(e > 126 ? 126 : e) : 1.f, down = 1.f / up;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *factor = up;
-    for (int64_t t = blockIdx.x * (int64_t)kThreads + threadIdx.x; t < T_; t += (int64_t)gridDim.x * kThreads) row_factor[t] = grad_loss[t] * down;
-}
-
+// ---- backward ------------------------------------------------------------------------------
 __device__ __forceinline__ void store(void *p, int type, int64_t i, float v) {
     if (type == MSD_F32) ((float *)p)[i] = v;
     else if (type == MSD_BF16) ((__nv_bfloat16 *)p)[i] = __float2bfloat16_rn(v);
@@ -302,15 +282,19 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 // ---- host -----------------------------------------------------------------------------------
 struct Plan {
     int P;               // pieces of an operand
+    bool joins;          // 16-bit gradients of products in pieces: always in partial sums that are joined
     int64_t T, C, O, ld;  // tokens, channels, labels, channels as packed
     bool pack_w;
     int64_t chunk, chunks;  // tokens at a time: the packed features of more than 512 MB are not held at once
     int64_t pieces, width;  // label pieces of the backward pass
 };
 
-static Plan make_plan(const Problem &p) {
+// `backward`: of the products with G.  Weights per token may span many orders of magnitude, and one float16
+// holds G over few of them: with such weights float16 goes through the three pieces too.
+static Plan make_plan(const Problem &p, bool backward) {
     Plan q;
-    q.P = p.dtype == MSD_F32 ? 3 : 1;
+    q.P = p.dtype == MSD_F32 || (backward && p.dtype == MSD_F16 && p.reduction == MSD_REDUCE_NONE) ? 3 : 1;
+    q.joins = q.P > 1 && p.dtype != MSD_F32;
     q.T = p.x.tokens(), q.C = p.x.C, q.O = p.labels;
     q.ld = round_up(q.C, 8);
     q.pack_w = q.P > 1 || q.C % 8 || ((uintptr_t)p.weight & 15);
@@ -380,8 +364,7 @@ static ForwardSpace carve_forward(const Plan &q, Carver *c) {
 
 struct BackwardSpace {
     uint16_t *g;
-    uint32_t *words;  // [0]: magnitude of the upstream gradient; [1] as float: its factor
-    float *run, *columns, *row_factor, *part[2];
+    float *run, *columns, *part[2];
     float *run_w;    // several chunks: sums of dW and db
     double *run_b;
 };
@@ -396,16 +379,14 @@ static void choose_splits(const Plan &q, int64_t tokens, int64_t labels, int pai
     *sx = (int)ceil_div(kx, share), *sw = (int)ceil_div(kw, share);
 }
 
-static BackwardSpace carve_backward(const Plan &q, int reduction, Carver *c) {
+static BackwardSpace carve_backward(const Plan &q, Carver *c) {
     BackwardSpace b;
-    b.words = c->take<uint32_t>(64);
     b.g = c->take<uint16_t>(q.P * q.chunk * q.width);
     const int64_t ld = round_up(q.C, 4);
     b.run = q.pieces > 1 ? c->take<float>(q.chunk * ld) : nullptr;
     b.run_w = q.chunks > 1 ? c->take<float>(q.O * ld) : nullptr;
     b.run_b = q.chunks > 1 ? c->take<double>(q.O) : nullptr;
     b.columns = c->take<float>(ceil_div(q.chunk, 32) * q.width);
-    b.row_factor = reduction == MSD_REDUCE_NONE ? c->take<float>(q.T) : nullptr;
     size_t most[2] = {0, 0};
     // chunks and pieces in the middle are like the first
     const int64_t tokens[2] = {q.chunk, q.T - (q.chunks - 1) * q.chunk}, labels[2] = {q.O < q.width ? q.O : q.width, q.O - (q.pieces - 1) * q.width};
@@ -413,7 +394,7 @@ static BackwardSpace carve_backward(const Plan &q, int reduction, Carver *c) {
         const int64_t t = tokens[i & 1], w = labels[i >> 1];
         int s[2];
         choose_splits(q, t, w, kMaxPairs, &s[0], &s[1]);
-        const size_t n[2] = {s[0] > 1 ? (size_t)s[0] * t * ld : 0, s[1] > 1 ? (size_t)s[1] * w * ld : 0};
+        const size_t n[2] = {s[0] > 1 || q.joins ? (size_t)s[0] * t * ld : 0, s[1] > 1 || q.joins ? (size_t)s[1] * w * ld : 0};
         for (int k = 0; k < 2; ++k) most[k] = n[k] > most[k] ? n[k] : most[k];
     }
     for (int i = 0; i < 2; ++i) b.part[i] = most[i] ? c->take<float>(most[i]) : nullptr;
@@ -423,24 +404,36 @@ static BackwardSpace carve_backward(const Plan &q, int reduction, Carver *c) {
 size_t forward_workspace_bytes(const Problem &p) {
     if (narrow_supported(p)) return narrow_workspace_bytes(p);
     Carver c(nullptr);
-    const Plan q = make_plan(p);
+    const Plan q = make_plan(p, false);
     carve_forward(q, &c);
     carve_operands(q, &c);
     return c.used + 256;
 }
 
-// A backward call after few_forward packs the operands itself.
+// Whether the forward call left the operands as the backward call takes them.  (few_forward packs none.)
+static bool kept_by_forward(const Problem &p, const Plan &backward) {
+    const Plan f = make_plan(p, false);
+    return f.P == backward.P && keeps_operands(f) && !few_supported(p);
+}
+
+// Enough for every reduction.
 size_t backward_workspace_bytes(const Problem &p) {
     if (narrow_supported(p)) return narrow_workspace_bytes(p);
-    Carver c(nullptr);
-    const Plan q = make_plan(p);
-    carve_backward(q, MSD_REDUCE_NONE, &c);
-    if (!keeps_operands(q) || few_supported(p)) carve_operands(q, &c);
-    return c.used + 256;
+    size_t most = 0;
+    Problem r = p;
+    for (int reduction : {MSD_REDUCE_NONE, MSD_REDUCE_MEAN}) {
+        r.reduction = reduction;
+        Carver c(nullptr);
+        const Plan q = make_plan(r, true);
+        carve_backward(q, &c);
+        if (!kept_by_forward(r, q)) carve_operands(q, &c);
+        if (c.used > most) most = c.used;
+    }
+    return most + 256;
 }
 
 size_t saved_bytes(const Problem &p) {
-    const Plan q = make_plan(p);
+    const Plan q = make_plan(p, false);
     if (narrow_supported(p) || few_supported(p)) return stats_bytes(q);
     Carver c(nullptr);
     if (keeps_operands(q)) carve_operands(q, &c);
@@ -473,6 +466,7 @@ static int pack_operands(const Problem &p, const Plan &q, const Operands &op, in
     k.blocks_x = bx;
     const unsigned grid = (unsigned)(bx + bw);
     if (p.dtype == MSD_F32) pack_kernel<float, 3><<<grid, kThreads, 0, s>>>(k);
+    else if (q.P > 1) pack_kernel<__half, 3><<<grid, kThreads, 0, s>>>(k);
     else if (p.dtype == MSD_BF16) pack_kernel<__nv_bfloat16, 1><<<grid, kThreads, 0, s>>>(k);
     else pack_kernel<__half, 1><<<grid, kThreads, 0, s>>>(k);
     return launched();
@@ -551,7 +545,7 @@ static int few_forward(const Problem &p, float *loss, float *saved, float2 *part
 
 int forward(const Problem &p, float *loss, float *saved, void *ws, size_t wsb, int device, cudaStream_t s) {
     if (narrow_supported(p)) return narrow_forward(p, loss, saved, ws, wsb, device, s);
-    const Plan q = make_plan(p);
+    const Plan q = make_plan(p, false);
     Carver c(ws);
     const ForwardSpace f = carve_forward(q, &c);
     Operands op = carve_operands(q, &c);
@@ -624,8 +618,8 @@ static void assign(MmaParams *m, int pairs, bool use0, bool use1) {
 }
 
 // Gradients from the tokens [t0, t0 + T_) and the labels [o0, o0 + width): G, then the sums over it.
-static int backward_piece(const Problem &p, const Plan &q, const Operands &op, const BackwardSpace &b, const float *saved, const Factor &factor, int64_t t0,
-                          int64_t T_, int64_t o0, const Features *dx, void *dw, void *db, int device, int pairs, cudaStream_t s) {
+static int backward_piece(const Problem &p, const Plan &q, const Operands &op, const BackwardSpace &b, const Stats &stats, const float *row_factor, const Factor &factor,
+                          int64_t t0, int64_t T_, int64_t o0, const Features *dx, void *dw, void *db, int device, int pairs, cudaStream_t s) {
     const size_t esize = p.dtype == MSD_F32 ? 4 : 2;
     const int64_t n = q.O - o0 < q.width ? q.O - o0 : q.width, gw = round_up(n, 64), g_piece = T_ * gw;
     const uint16_t *w = q.pack_w ? op.w : (const uint16_t *)p.weight;
@@ -634,11 +628,11 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     XENT_TRY(common_params(p, q, op, t0, device, &m));
     XENT_TRY(logit_product(p, q, op, T_, o0, n, pairs, &m.p[0]));
     m.label0 = (int)o0;
-    m.stats = Stats::of(const_cast<float *>(saved), q.T).at(t0), m.row_factor = b.row_factor ? b.row_factor + t0 : nullptr, m.factor = factor;
+    m.stats = stats.at(t0), m.row_factor = row_factor ? row_factor + t0 : nullptr, m.factor = factor;
     m.columns = db ? b.columns : nullptr;
     m.g = b.g, m.g_width = gw, m.g_piece = g_piece;
     // |G| <= 2 in units of the factor: one float16 holds it times 2^14, down to 2^-38
-    m.g_scale = p.dtype == MSD_F16 ? 16384.f : 1.f;
+    m.g_scale = p.dtype == MSD_F16 && q.P == 1 ? 16384.f : 1.f;
     const int64_t tiles = (int64_t)m.p[0].tiles_m * m.p[0].tiles_n;
     XENT_TRY(launch_mma<kGrad>(m, q.P, (int)(tiles < pairs ? tiles : pairs), s));
     if (db) {
@@ -670,7 +664,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
         r.tile_n = kTileN;
         r.tiles_m = (int)ceil_div(r.M, kTileM), r.tiles_n = (int)ceil_div(r.N, kTileN);
         r.k_blocks = (int)ceil_div(r.K, kDepth), r.splits = splits[i];
-        r.part = b.part[i];
+        r.parts = r.splits > 1 || q.joins, r.part = b.part[i];
         r.ld = (int)round_up(r.N, 4);
         const int64_t e = 16 / (int64_t)esize;
         r.linear = r.V >= r.row0 + r.M;
@@ -681,7 +675,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     assign(&m, pairs, dx != nullptr, dw != nullptr);
     XENT_TRY(launch_mma<kBack>(m, q.P, pairs, s));
     for (int i = 0; i < 2; ++i)
-        if (m.p[i].splits > 1 && (i == 0 ? dx != nullptr : dw != nullptr)) {
+        if (m.p[i].parts && (i == 0 ? dx != nullptr : dw != nullptr)) {
             join_kernel<<<(unsigned)ceil_div((int64_t)m.p[i].M * m.p[i].N, m.p[i].splits <= kFewSplits ? kThreads : 32), kThreads, 0, s>>>(m, i, p.dtype);
             XENT_TRY(launched());
         }
@@ -691,7 +685,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
 int backward(const Problem &p, const float *saved, const float *grad_loss, const Features *dx, void *dw, void *db, void *ws, size_t wsb, int device,
              cudaStream_t s) {
     if (narrow_supported(p) && (dx || dw || db)) return narrow_backward(p, nullptr, const_cast<float *>(saved), grad_loss, dx, dw, db, ws, wsb, device, s);
-    const Plan q = make_plan(p);
+    const Plan q = make_plan(p, true);
     const size_t esize = p.dtype == MSD_F32 ? 4 : 2;
     if (q.T == 0) {
         if (dw) MSD_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)q.O * q.C * esize, s));
@@ -700,29 +694,21 @@ int backward(const Problem &p, const float *saved, const float *grad_loss, const
     }
     if (!dx && !dw && !db) return MSD_OK;
     Carver c(ws);
-    const BackwardSpace b = carve_backward(q, p.reduction, &c);
+    const BackwardSpace b = carve_backward(q, &c);
     if (!ws || wsb < c.used) MSD_FAIL(MSD_ERR_WORKSPACE, "linear cross entropy backward: workspace of %zu bytes needed, %zu given", c.used, wsb);
     const int sms = fast::sm_count(device), pairs = pair_count(sms);
-    const bool kept = keeps_operands(q) && !few_supported(p);
+    const bool kept = kept_by_forward(p, q), per_token = p.reduction == MSD_REDUCE_NONE;
     Carver k(kept ? (char *)const_cast<float *>(saved) + stats_bytes(q) : (char *)ws + c.used);
     const Operands op = carve_operands(q, &k);
     if (!kept) {
         if (wsb < c.used + k.used) MSD_FAIL(MSD_ERR_WORKSPACE, "linear cross entropy backward: workspace of %zu bytes needed, %zu given", c.used + k.used, wsb);
     }
-    Factor factor{grad_loss, Stats::of(const_cast<float *>(saved), q.T).factor};
-    if (b.row_factor) {
-        const int64_t row_blocks = ceil_div(q.T, 4 * kThreads) < sms * 8 ? ceil_div(q.T, 4 * kThreads) : sms * 8;
-        MSD_CUDA_TRY(cudaMemsetAsync(b.words, 0, 8, s));
-        upstream_max_kernel<<<(unsigned)row_blocks, kThreads, 0, s>>>(grad_loss, p.target, p.ignore_index, q.T, b.words);
-        XENT_TRY(launched());
-        factor = Factor{(const float *)(b.words + 1), nullptr};
-        factor_kernel<<<(unsigned)row_blocks, kThreads, 0, s>>>(grad_loss, q.T, b.words, b.row_factor, (float *)(b.words + 1));
-        XENT_TRY(launched());
-    }
+    const Stats stats = Stats::of(const_cast<float *>(saved), q.T);
+    const Factor factor = per_token ? Factor{nullptr, nullptr} : Factor{grad_loss, stats.factor};
     for (int64_t t0 = 0; t0 < q.T; t0 += q.chunk) {
         const int64_t T_ = q.T - t0 < q.chunk ? q.T - t0 : q.chunk;
         if (!kept) XENT_TRY(pack_operands(p, q, op, t0, T_, s));
-        for (int64_t o0 = 0; o0 < q.O; o0 += q.width) XENT_TRY(backward_piece(p, q, op, b, saved, factor, t0, T_, o0, dx, dw, db, device, pairs, s));
+        for (int64_t o0 = 0; o0 < q.O; o0 += q.width) XENT_TRY(backward_piece(p, q, op, b, stats, per_token ? grad_loss : nullptr, factor, t0, T_, o0, dx, dw, db, device, pairs, s));
     }
     return MSD_OK;
 }

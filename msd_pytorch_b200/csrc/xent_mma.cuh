@@ -62,7 +62,8 @@ struct Product {
     int tile_n;                // columns of a tile: 256, or 192 or 128 where that fills the GPU better
     int splits, k_blocks;      // the contraction in blocks of 64, cut into `splits` ranges
     bool a_mn, b_mn;           // operand stored with m / n innermost instead of k
-    float *part;               // splits > 1: [split][M][ld] partial sums
+    bool parts;                // results go to `part`, to be joined, scaled and rounded later
+    float *part;               // [split][M][ld] partial sums
     float *sum;                // [M][ld]: running float32 result over several pieces of the labels, or null
     int ld;                    // N rounded up to a multiple of 4
     bool add, last;            // add `sum` to the product; write `out` (else `sum`)
@@ -73,10 +74,10 @@ struct Product {
     int64_t V, sn, sm, sc, row0;
 };
 
-// What the gradients are multiplied with: the product of one or two values on the device.
+// What the gradients are multiplied with: the product of two values on the device, or nothing.
 struct Factor {
     const float *a, *b;
-    __device__ __forceinline__ float value() const { return b ? *a * *b : *a; }
+    __device__ __forceinline__ float value() const { return a ? *a * *b : 1.f; }
 };
 
 struct MmaParams {
@@ -102,15 +103,6 @@ struct MmaParams {
     int first[2][kMaxPairs + 1];
     int *status;
 };
-
-// s with v s in [2^14, 2^15) for the largest magnitude v (1 for 0); exact.
-__device__ __forceinline__ int scale_exponent(uint32_t max_bits) {
-    const int e = (int)(max_bits >> 23);  // 0 for zero and subnormals
-    if (max_bits == 0) return 0;
-    int s = 14 - (e - 127);
-    return s > 126 ? 126 : s;
-}
-__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -512,7 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
             } else {
                 const bool ok = !*abort_flag, live = row < q.M && ok;
                 const float f = p.factor.value() / p.g_scale;
-                const bool split = q.splits > 1, done = !split && q.last;
+                const bool split = q.parts, done = !split && q.last;
                 float *run = split ? q.part + ((int64_t)it.split * q.M + row) * q.ld : q.sum + (int64_t)row * q.ld;
                 const bool add = !split && q.add;
                 const int64_t at = q.linear ? (q.row0 + row) * q.sm : ((q.row0 + row) / q.V) * q.sn + ((q.row0 + row) % q.V) * q.sm;

@@ -94,3 +94,41 @@ def test_token_weights_of_all_sizes(cuda_device, shape, O):
     weights = 10.0 ** torch.linspace(-9, 9, y.numel(), device=cuda_device).view(y.shape)
     check(x, w, b, y, weights)
     check(x, w, b, y, torch.flip(weights, [0]))
+
+
+@pytest.mark.parametrize("size", [3.4028e38, 1e-30])
+def test_ends_of_the_range(cuda_device, size):
+    """Features up to the largest float32 (which no bfloat16 is as large as), and close to the smallest."""
+    x, w, b, y = make((150, 40), 70, torch.float32, 53, cuda_device, ignored=0.1)
+    x = x.clamp(-1, 1) * size
+    check(x, w / size, b, y, torch.ones(y.shape, device=cuda_device)) if size < 1 else check(x, w * 1e-38, b, y, torch.full(y.shape, 2.0 ** -60, device=cuda_device))
+
+
+@pytest.mark.parametrize("dtype,lo,hi", [(torch.bfloat16, -9, 9), (torch.float16, -6, 2)], ids=str)
+@pytest.mark.parametrize("shape,O", SHAPES, ids=lambda v: str(v).replace(" ", ""))
+def test_token_weights_in_16_bits(cuda_device, shape, O, dtype, lo, hi):
+    """The same with 16-bit features (float16's own smallest step beside the bound)."""
+    x, w, b, y = make(shape, O, dtype, 54, cuda_device, ignored=0.1)
+    weights = 10.0 ** torch.linspace(lo, hi, y.numel(), device=cuda_device).view(y.shape)
+    floor = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    check(x, w, b, y, weights, floor)
+    check(x, w, b, y, torch.flip(weights, [0]), floor)
+
+
+@pytest.mark.parametrize("T,C,O", [(1500, 300, 700), (40, 24, 150001), (5000, 24, 9)])
+def test_token_weights_in_float16_by_size(cuda_device, T, C, O):
+    """Several splits of the contraction, several pieces of the labels, few labels over rows."""
+    x, w, b, y = make((T, C), O, torch.float16, 55, cuda_device, ignored=0.1)
+    weights = 10.0 ** torch.linspace(-6, 0, T, device=cuda_device)
+    check(x, w, b, y, weights, 2.0 ** -25)
+
+
+@pytest.mark.parametrize("shape,O", SHAPES, ids=lambda v: str(v).replace(" ", ""))
+def test_one_heavy_token_in_float16(cuda_device, shape, O):
+    """A token of weight 6e4 takes nothing from the features' gradients of tokens of weight 1e-4."""
+    x, w, b, y = make(shape, O, torch.float16, 56, cuda_device, ignored=0.0)
+    first = x[0, :, ...].reshape(shape[1], -1)[:, 0] if x.dim() > 2 else x[0]
+    first.mul_(0.1)
+    weights = torch.full(y.shape, 1e-4, device=cuda_device)
+    weights.view(-1)[0] = 6e4
+    check(x, w, b, y, weights, 2.0 ** -25)
