@@ -19,7 +19,8 @@ namespace xent {
 
 constexpr int kThreads = 256;
 constexpr int kCombineBlocks = 592;
-constexpr int64_t kPieceBytes = 256ll << 20;  // G held at a time
+constexpr int64_t kPieceBytes = 256ll << 20;  // G held at a time (half as much again where that saves a piece)
+constexpr int64_t kPieceLabels = 256;         // labels of a piece, at least (fewer only if there are no more)
 constexpr int64_t kChunkBytes = 512ll << 20;  // packed features held at a time
 
 static size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
@@ -285,7 +286,7 @@ struct Plan {
     bool joins;          // 16-bit gradients of products in pieces: always in partial sums that are joined
     int64_t T, C, O, ld;  // tokens, channels, labels, channels as packed
     bool pack_w;
-    int64_t chunk, chunks;  // tokens at a time: the packed features of more than 512 MB are not held at once
+    int64_t chunk, chunks;  // tokens at a time: neither more than 512 MB of packed features, nor a piece of G above its limit
     int64_t pieces, width;  // label pieces of the backward pass
 };
 
@@ -298,13 +299,15 @@ static Plan make_plan(const Problem &p, bool backward) {
     q.T = p.x.tokens(), q.C = p.x.C, q.O = p.labels;
     q.ld = round_up(q.C, 8);
     q.pack_w = q.P > 1 || q.C % 8 || ((uintptr_t)p.weight & 15);
-    q.chunk = kChunkBytes / (2 * q.P * q.ld) / kTileM * kTileM;
+    const int64_t g_labels = q.O < kPieceLabels ? round_up(q.O, 64) : kPieceLabels;
+    const int64_t by_x = kChunkBytes / (2 * q.P * q.ld), by_g = kPieceBytes / (2 * q.P * g_labels);
+    q.chunk = (by_x < by_g ? by_x : by_g) / kTileM * kTileM;
     if (q.chunk < 16 * kTileM) q.chunk = 16 * kTileM;
     if (q.chunk > q.T) q.chunk = q.T;
     q.chunks = q.T ? ceil_div(q.T, q.chunk) : 0;
     const int64_t per_label = (q.T ? q.chunk : 1) * 2 * q.P;
     int64_t most = kPieceBytes / per_label;
-    if (most < 256) most = 256;
+    if (most < kPieceLabels) most = kPieceLabels;
     q.pieces = (q.O + most / 2) / most;
     if (q.pieces < 1) q.pieces = 1;
     q.width = round_up(ceil_div(q.O, q.pieces), 64);
