@@ -437,7 +437,8 @@ size_t backward_workspace_bytes(const Problem &p) {
 
 size_t saved_bytes(const Problem &p) {
     const Plan q = make_plan(p, false);
-    if (narrow_supported(p) || few_supported(p)) return stats_bytes(q);
+    if (narrow_supported(p)) return 256;
+    if (few_supported(p)) return stats_bytes(q);
     Carver c(nullptr);
     if (keeps_operands(q)) carve_operands(q, &c);
     return stats_bytes(q) + c.used;

@@ -79,6 +79,7 @@ struct Problem {
 bool narrow_supported(const Problem &p);
 bool single_pass(const Problem &p);
 size_t narrow_workspace_bytes(const Problem &p);
+// stats: one float, the factor of the reduction
 int narrow_forward(const Problem &p, float *loss, float *stats, void *ws, size_t wsb, int device, cudaStream_t s);
 // loss non-null: writes it too (mean or sum) and takes the upstream gradient as 1
 int narrow_backward(const Problem &p, float *loss, float *stats, const float *grad_loss, const Features *dx, void *dw, void *db, void *ws, size_t wsb,

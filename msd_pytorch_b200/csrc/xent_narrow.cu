@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(1024) count_kernel(const int64_t *target, int6
 // Adds up the blocks' sums: 32 outputs x 8 lanes per block.  Block 0 also finishes the loss.
 template <typename T>
 __global__ void __launch_bounds__(256) narrow_finish_kernel(const float *part, int blocks, int64_t weights, int64_t outputs, T *dw, T *db, const double *block_sum,
-                                                            const int64_t *block_count, int reduction, int64_t T_, float *loss, float *stats) {
+                                                            const int64_t *block_count, int reduction, float *loss, float *stats) {
     __shared__ double red[8][33];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
     const int64_t i = blockIdx.x * 32ll + x;
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) narrow_finish_kernel(const float *part, i
         }
         if (x == 0) {
             loss[0] = (float)(reduction == MSD_REDUCE_MEAN ? total / (double)count : total);
-            stats[T_] = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
+            stats[0] = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
         }
     }
 }
@@ -110,7 +110,7 @@ size_t narrow_workspace_bytes(const Problem &p) {
     return carve_narrow(p, nullptr, &n) + 256;
 }
 
-__global__ void loss_finish_kernel(const double *block_sum, const int64_t *block_count, int blocks, int reduction, int64_t T_, float *loss, float *stats) {
+__global__ void loss_finish_kernel(const double *block_sum, const int64_t *block_count, int blocks, int reduction, float *loss, float *stats) {
     double total = 0;
     int64_t count = 0;
     for (int b = threadIdx.x; b < blocks; b += 32) total += block_sum[b], count += block_count[b];
@@ -122,7 +122,7 @@ __global__ void loss_finish_kernel(const double *block_sum, const int64_t *block
     if (threadIdx.x) return;
     if (reduction == MSD_REDUCE_MEAN) loss[0] = (float)(total / (double)count);
     if (reduction == MSD_REDUCE_SUM) loss[0] = (float)total;
-    if (stats) stats[T_] = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
+    if (stats) stats[0] = reduction == MSD_REDUCE_MEAN ? (count ? (float)(1.0 / (double)count) : 0.f) : 1.f;
 }
 
 static void fill(const Problem &p, const NarrowSpace &n, NarrowParams *q) {
@@ -222,7 +222,7 @@ int narrow_forward(const Problem &p, float *loss, float *stats, void *ws, size_t
     q.losses = p.reduction == MSD_REDUCE_NONE ? loss : nullptr;
     int blocks = 0, rc;
     if ((rc = dispatch(p, q, rows_aligned(p.x, p.dtype == MSD_F32 ? 4 : 2), false, device, &blocks, s))) return rc;
-    loss_finish_kernel<<<1, 32, 0, s>>>(n.bsum, n.bcount, blocks, p.reduction, p.x.tokens(), loss, stats);
+    loss_finish_kernel<<<1, 32, 0, s>>>(n.bsum, n.bcount, blocks, p.reduction, loss, stats);
     return narrow_launched();
 }
 
@@ -253,19 +253,19 @@ int narrow_backward(const Problem &p, float *loss, float *stats, const float *gr
         const int rc = narrow_launched();
         if (rc) return rc;
     } else if (q.mean) {
-        q.mean_factor = stats + T_;
+        q.mean_factor = stats;
     }
     int blocks = 0, rc;
     if ((rc = dispatch(p, q, aligned, true, device, &blocks, s))) return rc;
     const int64_t weights = p.labels * p.x.C, outputs = weights + p.labels;
     const unsigned grid = (unsigned)ceil_div(outputs, 32);
     if (p.dtype == MSD_F32)
-        narrow_finish_kernel<float><<<grid, 256, 0, s>>>(n.part, blocks, weights, outputs, (float *)dw, (float *)db, n.bsum, n.bcount, p.reduction, T_, loss, stats);
+        narrow_finish_kernel<float><<<grid, 256, 0, s>>>(n.part, blocks, weights, outputs, (float *)dw, (float *)db, n.bsum, n.bcount, p.reduction, loss, stats);
     else if (p.dtype == MSD_BF16)
         narrow_finish_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(n.part, blocks, weights, outputs, (__nv_bfloat16 *)dw, (__nv_bfloat16 *)db, n.bsum, n.bcount,
-                                                                 p.reduction, T_, loss, stats);
+                                                                 p.reduction, loss, stats);
     else
-        narrow_finish_kernel<__half><<<grid, 256, 0, s>>>(n.part, blocks, weights, outputs, (__half *)dw, (__half *)db, n.bsum, n.bcount, p.reduction, T_, loss,
+        narrow_finish_kernel<__half><<<grid, 256, 0, s>>>(n.part, blocks, weights, outputs, (__half *)dw, (__half *)db, n.bsum, n.bcount, p.reduction, loss,
                                                           stats);
     return narrow_launched();
 }

@@ -51,7 +51,7 @@ struct NarrowParams {
     bool want_dx;
     const float *grad_loss;  // null: 1
     bool per_token;          // grad_loss per token
-    const float *mean_factor;  // factor of a mean (stats[tokens]), or null
+    const float *mean_factor;  // factor of a mean (what forward left), or null
     const int64_t *counted;    // instead: the number of tokens that count,
     int count_here;            // or, above 0, every block counts the targets itself
     bool mean;

@@ -28,3 +28,10 @@ def test_work_space_is_bounded(dtype, channels, voxels, labels):
     logits = 4 * voxels * labels
     if logits > 2048 * MB:
         assert max(forward, backward) < logits / 2
+
+
+@pytest.mark.parametrize("dtype", [_lib.MSD_F32, _lib.MSD_BF16, _lib.MSD_F16])
+def test_few_labels_keep_nothing_per_voxel(dtype):
+    """The backward pass of few labels computes its statistics again."""
+    for voxels in (64, 128 ** 3):
+        assert sizes(dtype, 2, 51, voxels, 11)[0] <= 256
