@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 #include <string.h>
+#include <atomic>
 #include "xent.h"
 
 namespace msd {
@@ -176,7 +177,14 @@ template <typename T, int N>
 static int launch_few_tokens(const FewParams &p, int blocks, cudaStream_t s) {
     auto kern = p.vec ? few_kernel<T, N, true> : few_kernel<T, N, false>;
     const size_t smem = (size_t)N * p.C4 * sizeof(float);
-    MSD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // the most that any call takes, once: the limit is shared by all threads of the process
+    static std::atomic<uint64_t> ready[2];
+    int device = 0;
+    MSD_CUDA_TRY(cudaGetDevice(&device));
+    if (device >= 64 || !(ready[p.vec].load() >> device & 1)) {
+        MSD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(N * kFewChannels * sizeof(float))));
+        if (device < 64) ready[p.vec].fetch_or(1ull << device);
+    }
     kern<<<blocks, 32 * kFewWarps, smem, s>>>(p);
     MSD_CUDA_TRY(cudaGetLastError());
     return MSD_OK;
