@@ -156,6 +156,11 @@ def _empty_gradient(x, x_geometry):
     return grad, geometry
 
 
+def capturing(x):
+    """Whether this thread's work on the device of ``x`` is being captured into a graph."""
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def scale_(tensors, factor):
     """Multiplies dense tensors in place with the float32 value of ``factor`` (0-dimensional, on the device)."""
     table = array.array("q")
@@ -193,7 +198,8 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
     """With few labels over float32 images or volumes the gradients are computed in the forward pass,
     with the loss: x, which everything is bound by, is then read once instead of twice.  The
     backward pass multiplies them with the upstream gradient (nothing to do for 1) and hands
-    them out; a second backward pass of a kept graph computes them again."""
+    them out; a second backward pass of a kept graph computes them again, and so does one that is captured
+    when the forward pass was not (its replays would multiply the same values again and again)."""
 
     @staticmethod
     def forward(ctx, input, weight, bias, target, ignore_index, reduction):
@@ -205,7 +211,7 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
             grad_weight = torch.empty_like(weight) if need[1] else None
             grad_bias = torch.empty_like(bias) if bias is not None and need[2] else None
             loss, saved = xent_step_(input, geometry, weight, bias, target, ignore_index, reduction, grad_x, grad_geometry, grad_weight, grad_bias)
-            ctx.grads = (grad_x, grad_weight, grad_bias)
+            ctx.grads, ctx.captured = (grad_x, grad_weight, grad_bias), capturing(input)
         else:
             loss, saved = xent_forward_(input, geometry, weight, bias, target, ignore_index, reduction, True)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
@@ -217,8 +223,8 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_loss):
         input, weight, bias, target, saved = ctx.saved_tensors
-        if ctx.grads is not None:
-            grads, ctx.grads = ctx.grads, None
+        grads, ctx.grads = ctx.grads, None
+        if grads is not None and (ctx.captured or not capturing(input)):
             scale_([g for g in grads if g is not None], grad_loss)
             return (*grads, None, None, None)
         # hooks on saved tensors may hand them back in another layout

@@ -200,7 +200,7 @@ class MSDModuleLossFunction(torch.autograd.Function):
         if wanted and losses.single_pass(result, geometry, fw.shape[0]):
             gradients, gfw, gfb = torch.empty_like(result), torch.empty_like(fw), torch.empty_like(fb)
             loss, saved = losses.xent_step_(result, geometry, fw, fb, target, ignore_index, "mean", gradients, geometry, gfw, gfb)
-            ctx.gradients = (gradients, gfw, gfb)
+            ctx.gradients, ctx.captured = (gradients, gfw, gfb), losses.capturing(input)
         else:
             loss, saved = losses.xent_forward_(result, geometry, fw, fb, target, ignore_index, "mean", wanted)
         ctx.dilations, ctx.c_in, ctx.w_in, ctx.ignore_index = list(dilations), c_in, w_in, ignore_index
@@ -212,8 +212,9 @@ class MSDModuleLossFunction(torch.autograd.Function):
     def backward(ctx, grad_loss):
         bias, result, fw, fb, final_weight, target, saved, *weights = ctx.saved_tensors
         result = result.contiguous()  # hooks on saved tensors may hand it back in another layout
-        if ctx.gradients is not None:
-            (gradients, gfw, gfb), ctx.gradients = ctx.gradients, None
+        ready, ctx.gradients = ctx.gradients, None
+        if ready is not None and (ctx.captured or not losses.capturing(result)):  # see LinearCrossEntropyFunction
+            gradients, gfw, gfb = ready
             losses.scale_([gradients, gfw, gfb], grad_loss)
         else:
             gradients, gfw, gfb = torch.empty_like(result), torch.empty_like(fw), torch.empty_like(fb)
