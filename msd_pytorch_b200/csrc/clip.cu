@@ -187,16 +187,30 @@ __global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double *par
     }
 }
 
+// The factor, for float32 arithmetic as before * f: one factor f unless it is no normal float32 (values near
+// 1e38 clipped to a small norm).  Then `before` is a power of two that leaves f near 2^-30, and what it
+// makes subnormal of a value ends below the smallest float32 anyway.
+struct Scale {
+    double exact;
+    float before, f;
+    __device__ __forceinline__ explicit Scale(double v) : exact(v), before(1.f), f((float)v) {
+        if (v > 0 && v < 0x1p-126) {
+            const int k = min(-30 - ilogb(v), 126);
+            before = scalbnf(1.f, -k), f = (float)scalbn(v, k);
+        }
+    }
+    __device__ __forceinline__ float operator()(float v) const { return v * before * f; }
+};
 template <typename T>
-__device__ __forceinline__ T scaled(T v, double f) {
-    if constexpr (sizeof(T) == 8) return v * f;
-    else if constexpr (sizeof(T) == 4) return v * (float)f;
-    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(__bfloat162float(v) * (float)f);
-    else return __float2half_rn(__half2float(v) * (float)f);
+__device__ __forceinline__ T scaled(T v, const Scale &f) {
+    if constexpr (sizeof(T) == 8) return v * f.exact;
+    else if constexpr (sizeof(T) == 4) return f(v);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(f(__bfloat162float(v)));
+    else return __float2half_rn(f(__half2float(v)));
 }
 
 template <typename T>
-__device__ __forceinline__ void scale_chunk(const Entry &e, int chunk, double f) {
+__device__ __forceinline__ void scale_chunk(const Entry &e, int chunk, const Scale &f) {
     constexpr int E = 16 / sizeof(T);
     const T *in = (const T *)e.in;
     T *out = (T *)e.out;
@@ -252,15 +266,16 @@ __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constan
         f = max_norm / (n + 1e-6);
         f = f > 1.0 ? 1.0 : f;
     }
+    const Scale s(f);
     for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         const Entry &e = t.e[find(t, c)];
         if (f == 1.0 && e.in == e.out) continue;
         const int at = c - e.first_chunk;
         switch (e.dtype) {
-            case MSD_F32: scale_chunk<float>(e, at, f); break;
-            case MSD_F64: scale_chunk<double>(e, at, f); break;
-            case MSD_BF16: scale_chunk<__nv_bfloat16>(e, at, f); break;
-            default: scale_chunk<__half>(e, at, f); break;
+            case MSD_F32: scale_chunk<float>(e, at, s); break;
+            case MSD_F64: scale_chunk<double>(e, at, s); break;
+            case MSD_BF16: scale_chunk<__nv_bfloat16>(e, at, s); break;
+            default: scale_chunk<__half>(e, at, s); break;
         }
     }
 }
