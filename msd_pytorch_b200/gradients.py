@@ -147,6 +147,8 @@ def clip_norm_(tensors, max_norm, norm_type=2.0, error_if_nonfinite=False, out=N
             for w, o in zip(written, targets):
                 if w is not o:
                     o.copy_(w)
+        # written by address: graphs that saved one of them have to know
+        torch.autograd.graph.increment_version(targets)
     return norm
 
 

@@ -24,3 +24,29 @@ def test_factors_below_the_smallest_normal_number(cuda_device, dtype, max_norm):
     half = torch.finfo(dtype).eps / 2
     relative = half + (2.0 ** -50 if dtype == torch.float64 else 5 * 2.0 ** -24)
     assert bool(((t.double() - want).abs() <= relative * want.abs()).all())
+
+
+def test_autograd_sees_the_change(cuda_device):
+    """A graph that saved a tensor refuses to go backward after the tensor was clipped, as after any operation
+    in place; outputs count as written, inputs beside them do not."""
+    from msd_pytorch_b200 import clip_norm_
+
+    for strided in (False, True):
+        base = torch.randn(8, 6, device=cuda_device)
+        a, b = (base[:, ::2], torch.randn(5, device=cuda_device)) if strided else (base, torch.randn(5, device=cuda_device))
+        leaf = torch.randn(a.shape, device=cuda_device, requires_grad=True)
+        loss = (leaf * a).sum()
+        versions = a._version, b._version
+        clip_norm_([a, b], 0.1)
+        assert a._version > versions[0] and b._version > versions[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        out = [torch.empty_like(a), torch.empty_like(b)]
+        versions = a._version, b._version, out[0]._version, out[1]._version
+        clip_norm_([a, b], 0.1, out=out)
+        assert (a._version, b._version) == versions[:2]
+        assert out[0]._version > versions[2] and out[1]._version > versions[3]
+    with torch.inference_mode():  # tensors without a version
+        t = torch.ones(100, device=cuda_device)
+        clip_norm_([t], 1.0)
+        assert abs(float(t[0]) - 0.1) <= 1e-7
