@@ -10,7 +10,7 @@ from operator import attrgetter
 import torch
 
 from . import _lib
-from .losses import _scratch
+from .losses import _has_tangent, _scratch
 
 NORM_TYPES = {2.0: 0, float("inf"): 1}
 
@@ -42,6 +42,8 @@ def _dense(t):
 
 def _check_list(tensors, op):
     """Device and types of the tensors."""
+    if _has_tangent(*tensors):
+        raise RuntimeError("%s: forward-mode derivatives are not offered" % op)
     indices = set(map(_Tensor.get_device, tensors))
     if min(indices) < 0:
         raise RuntimeError("%s: expected CUDA tensors (there is no CPU implementation)" % op)
@@ -76,7 +78,8 @@ def _norm_tensor(dtypes, dev):
 
 def total_norm(tensors, norm_type=2.0):
     """The norm of all values of ``tensors`` taken together, as a 0-dimensional tensor on their
-    device (float32; float64 if every tensor is float64).  ``norm_type``: 2 or inf."""
+    device (float32; float64 if every tensor is float64).  ``norm_type``: 2 or inf.  A number to look at
+    or to clip by: no gradient flows through it."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
     if not tensors:
@@ -96,7 +99,7 @@ def clip_norm_(tensors, max_norm, norm_type=2.0, error_if_nonfinite=False, out=N
     :func:`total_norm`, and returns the norm.  In place, or, with ``out``, into the tensors listed
     there, with ``tensors`` left as they are: same types and shapes (contiguous ones may differ in
     shape, slices of a flat buffer for instance), no overlap with the input other than being the
-    same tensors.
+    same tensors.  A tensor that appears twice is refused: it would be scaled twice.
 
     Nothing waits for the GPU unless ``error_if_nonfinite`` is set, which raises a RuntimeError for a norm
     that is infinite or NaN and leaves the tensors unscaled."""
@@ -154,6 +157,6 @@ def clip_norm_(tensors, max_norm, norm_type=2.0, error_if_nonfinite=False, out=N
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """:func:`clip_norm_` of the gradients of ``parameters`` (those that have one), in place: the
-    calling convention of ``torch.nn.utils.clip_grad_norm_``."""
+    calling convention of ``torch.nn.utils.clip_grad_norm_``, but each parameter at most once."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     return clip_norm_([p.grad for p in parameters if p.grad is not None], max_norm, norm_type, error_if_nonfinite)

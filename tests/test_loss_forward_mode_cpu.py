@@ -1,4 +1,4 @@
-"""Forward-mode derivatives are not offered by the loss: a tangent is refused, not dropped."""
+"""Forward-mode derivatives are not offered by the loss and the clipping: a tangent is refused, not dropped."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -20,3 +20,16 @@ def test_tangents_are_refused(monkeypatch, which, grad):
             operands[which] = fwAD.make_dual(operands[which], torch.ones_like(operands[which]))
             with pytest.raises(RuntimeError, match="jvp"):
                 losses.linear_cross_entropy(*operands, y)
+
+
+def test_tangents_of_gradients_are_refused():
+    from msd_pytorch_b200 import clip_norm_, total_norm
+
+    t = torch.ones(3)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(t, torch.ones(3))
+        for call in (lambda: total_norm([t, dual]), lambda: clip_norm_([dual], 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="CUDA"):
+            total_norm([t])
