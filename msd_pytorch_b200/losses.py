@@ -90,6 +90,13 @@ def _check(input, weight, bias, target, reduction):
             raise RuntimeError("linear_cross_entropy: expected all tensors on %s, got one on %s" % (device, t.device))
 
 
+def _index(ignore_index):
+    index = int(ignore_index)
+    if not -2 ** 63 <= index < 2 ** 63:
+        raise ValueError("linear_cross_entropy: ignore_index must be a 64-bit integer, got %d" % index)
+    return index
+
+
 def xent_forward_(x, geometry, weight, bias, target, ignore_index, reduction, keep):
     """``(loss, saved)`` through the C ABI; the arguments have passed the checks and are dense."""
     dev = x.device
@@ -255,8 +262,9 @@ def linear_cross_entropy(input, weight, bias, target, ignore_index=-100, reducti
     NaN; a target that names no label makes the loss and the gradients that its token reaches NaN
     instead of ending the process."""
     _check(input, weight, bias, target, reduction)
+    ignore_index = _index(ignore_index)
     wanted = torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
     if not wanted and not _has_tangent(input, weight, bias):  # a tangent goes to autograd, which refuses it
         input, weight, bias, target, geometry = _operands(input, weight, bias, target)
-        return xent_forward_(input, geometry, weight, bias, target, int(ignore_index), reduction, False)[0]
-    return LinearCrossEntropyFunction.apply(input, weight, bias, target, int(ignore_index), reduction)
+        return xent_forward_(input, geometry, weight, bias, target, ignore_index, reduction, False)[0]
+    return LinearCrossEntropyFunction.apply(input, weight, bias, target, ignore_index, reduction)

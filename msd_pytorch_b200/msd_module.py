@@ -306,10 +306,11 @@ class MSDModule(torch.nn.Module):
         for t in (blk.bias, *weights):
             if t.device != input.device:
                 raise RuntimeError("MSDModule.cross_entropy: expected all tensors on %s, got one on %s" % (input.device, t.device))
+        ignore_index = losses._index(ignore_index)
         losses._check(input.detach()[:, :1], final.weight.detach()[:, :1], final.bias, target, "mean")
         if scale_in is not None and any(p.requires_grad for p in scale_in.parameters()):
             input, scale_in = scale_in(input), None
         # inside the node gradients are always off, and what its tensors require says nothing about no_grad
         wanted = torch.is_grad_enabled() and any(t.requires_grad for t in (input, blk.bias, final.weight, final.bias, *weights))
-        return MSDModuleLossFunction.apply(input.contiguous(), blk.dilations, blk.bias, final.weight, final.bias, target, int(ignore_index),
+        return MSDModuleLossFunction.apply(input.contiguous(), blk.dilations, blk.bias, final.weight, final.bias, target, ignore_index,
                                            None if scale_in is None else _scale_parts(scale_in), wanted, *weights)

@@ -44,3 +44,16 @@ def test_shapes():
     net.msd_block.bias = torch.nn.Parameter(torch.zeros(2))
     with pytest.raises(RuntimeError, match="3 block biases"):
         net.cross_entropy(x, y)
+
+
+@pytest.mark.parametrize("ignore", [2 ** 63, -2 ** 63 - 1, 2 ** 64 + 5])
+def test_ignore_index_out_of_range(monkeypatch, ignore):
+    """An index past 64 bits is refused instead of losing its high bits on the way to the library."""
+    from msd_pytorch_b200 import linear_cross_entropy, losses
+
+    monkeypatch.setattr(losses, "_check", lambda *a: None)
+    net, x, y = make()
+    with pytest.raises(ValueError, match="ignore_index"):
+        net.cross_entropy(x, y, ignore_index=ignore)
+    with pytest.raises(ValueError, match="ignore_index"):
+        linear_cross_entropy(torch.zeros(4, 3), torch.zeros(5, 3), None, torch.zeros(4, dtype=torch.int64), ignore_index=ignore)
