@@ -484,11 +484,9 @@ static int launch_mma(const MmaParams &m, int P, int pairs, cudaStream_t s) {
     int device = 0;
     MSD_CUDA_TRY(cudaGetDevice(&device));
     if (device >= 64 || !(ready[P > 1].load() >> device & 1)) {
-        if (P > 1) {
-            cudaFuncAttributes a;
-            MSD_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
-            if (a.numRegs < kRegsLaunch) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: built with %d registers per thread, %d expected", a.numRegs, kRegsLaunch);
-        }
+        cudaFuncAttributes a;
+        MSD_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
+        if (a.numRegs < kRegsLaunch) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: built with %d registers per thread, %d expected", a.numRegs, kRegsLaunch);
         MSD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (device < 64) ready[P > 1].fetch_or(1ull << device);
     }

@@ -14,9 +14,12 @@
 // step: one token of 1e8 took 8 bits from all others.)
 //
 // The tensor core's float32 additions truncate: a sum of n of them is off by up to n 2^-23 and
-// drifts towards zero (dW over 65536 tokens: 8e-6 off; a rounding sum 2e-7).  For float32 inputs
-// every 64 of the contraction is therefore a sum of its own, small products first, and the epilogue
-// warps add these sums in registers (rounding to nearest), under the products of the next 64.
+// drifts towards zero (a loss of 16-bit rows of 65536 channels: 4e-5 off, of 1000 channels 4e-7; a
+// rounding sum 1e-7).  So every stretch of the contraction is a sum of its own, small products first,
+// and the epilogue warps add these sums in registers (rounding to nearest), under the products of the next.
+// Float32 inputs: 64 at a time.  16-bit inputs: 1024 in logits, whatever their number (5e-7; 512 at a
+// time: 2.5e-7 and 6 % of a step of 4096 x 32768 x 1024, whose G has no time left for it), 4096 in
+// gradients, which are rounded to 16 bits.
 //
 // Two CTAs on neighbouring SMs work as a pair (cta_group::2) on tiles of 256 x 256: each loads its own
 // 128 rows of A and half of B, 32 KB per 64 of the contraction: 64 bytes per clock at the tensor core's
@@ -49,6 +52,8 @@ static_assert(kRegsIssue * 128 + kRegsEpilogue * 256 <= kRegsLaunch * kMmaThread
 
 enum Use { kLse = 0, kGrad = 1, kBack = 2 };
 
+// Blocks of 64 of the contraction whose products are added in the tensor core.
+__host__ __device__ constexpr int sum_blocks(int use, int pieces) { return pieces > 1 ? 1 : use == kBack ? 64 : 16; }
 __host__ __device__ constexpr int stages_of(int pieces) { return pieces == 1 ? 6 : 2; }
 __host__ __device__ constexpr size_t mma_smem_bytes(int pieces) {
     return 1024 + (size_t)stages_of(pieces) * pieces * (kABytes + kBBytes) + 2 * kTileN * sizeof(float) + 8 * 32 * kTurn * sizeof(float) + 256;
@@ -183,6 +188,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
     using namespace tma;
     static_assert(P == 1 || P == 3, "operands as they are, or in three pieces");
     constexpr bool WIDE = P > 1;
+    constexpr int F = sum_blocks(USE, P);  // a power of two
     constexpr int S = stages_of(P);
     constexpr int kStage = P * (kABytes + kBBytes);
     extern __shared__ unsigned char xent_smem[];
@@ -208,7 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
     // Three pieces: the epilogue warps keep 128 sums per thread.  kRegsIssue x 128 + kRegsEpilogue x 256 is
     // what the block was launched with (kRegsLaunch x 384; the launcher checks the compiled kernel).
     if (warp < 4) {
-        if (WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // The loops of both issuing warps run with all lanes (see umma::elect_one): with one lane in a
         // branch of its own the products of 64 took 1000 clocks to issue instead of the 512 they run.
         if (warp == 0) {
@@ -268,7 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 // 8192 bytes, 8 k at 1024, so 16 k = 2048 bytes.
                 const uint32_t a_step = q.a_mn ? 2048 / 16 : 32 / 16, b_step = q.b_mn ? 2048 / 16 : 32 / 16;
                 for (int kb = it.k0; kb < it.k1; ++kb) {
-                    const bool first = WIDE || kb == it.k0;
+                    const bool first = (kb - it.k0) % F == 0;
                     if (first) {
                         wait_parity(acc_empty + acc, acc_phase ^ 1, abort_flag, p.status, 22);
                         __syncwarp();
@@ -280,7 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     umma::fence_after_sync();
                     const uint32_t a = lo0 + (uint32_t)(stage * kStage) / 16, b = a + P * kABytes / 16;
                     const int steps = min(kDepth / 16, (K - kb * kDepth + 15) / 16);
-                    const bool sum_done = WIDE || kb + 1 == it.k1;
+                    const bool sum_done = (kb - it.k0) % F == F - 1 || kb + 1 == it.k1;
                     if (umma::elect_one()) {
                         // pieces whose orders add up to 2, then 1, then 0: the small products first
 #pragma unroll
@@ -304,14 +310,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
         }
         __syncwarp();
     } else {
-        if (WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         const int half = (warp - 4) >> 2, quad = warp & 3;
         Items<USE> items(p);
         Item it;
         int acc = 0;
         uint32_t acc_phase = 0;
         int parity = 0, biases_of = -1;
-        float run_sums[WIDE ? kTileN / 2 : 1];  // sums of the contraction so far
+        float run_sums[kTileN / 2];  // sums of the contraction so far
         while (items.get(it)) {
             const Product &q = p.p[it.which];
             const int row = it.m * kTileM + (int)rank * kCtaM + quad * 32 + lane;  // token (kBack, dW: label)
@@ -326,10 +332,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 p.stats.read(row, lse, rest);
                 if (p.row_factor) upstream = p.row_factor[row];
             }
-            if (WIDE) {
+            const bool several = WIDE || it.k1 - it.k0 > F;
+            if (several) {
 #pragma unroll
-                for (int j = 0; j < kTileN / 2; ++j) run_sums[WIDE ? j : 0] = 0.f;
-                for (int kb = it.k0; kb + 1 < it.k1; ++kb) {
+                for (int j = 0; j < kTileN / 2; ++j) run_sums[j] = 0.f;
+                for (int kb = it.k0; kb + F < it.k1; kb += F) {
                     wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 25);
                     __syncwarp();
                     umma::fence_after_sync();
@@ -341,7 +348,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                         umma::tmem_ld32_issue(t + c, r);
                         umma::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) run_sums[WIDE ? c + j : 0] += __uint_as_float(r[j]);
+                        for (int j = 0; j < 32; ++j) run_sums[c + j] += __uint_as_float(r[j]);
                     }
                     umma::fence_before_sync();
                     __syncwarp();
@@ -366,16 +373,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 float top = -CUDART_INF_F, sum = 0.f;
                 const bool live = in;
                 const int hit = live && y >= col0 && y < col0 + cols ? (int)(y - col0) : -1;
-#pragma unroll(WIDE ? 4 : 1)
+#pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
                     uint32_t r[32];
                     __syncwarp();
                     umma::tmem_ld32_issue(t0 + c, r);
                     umma::tmem_ld_wait();
-                    if (WIDE) {
+                    if (several) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[WIDE ? c + j : 0]);
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[c + j]);
                     }
                     float z[32], m = -CUDART_INF_F;
 #pragma unroll
@@ -417,16 +424,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 const int stored = (int)min((int64_t)width, p.g_width - col0);
                 const bool ok = !*abort_flag;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
-#pragma unroll(WIDE ? 4 : 1)
+#pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= stored) continue;
                     uint32_t r[32];
                     __syncwarp();
                     umma::tmem_ld32_issue(t0 + c, r);
                     umma::tmem_ld_wait();
-                    if (WIDE) {
+                    if (several) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[WIDE ? c + j : 0]);
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[c + j]);
                     }
                     float v[32];
 #pragma unroll
@@ -509,7 +516,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 const bool add = !split && q.add;
                 const int64_t at = q.linear ? (q.row0 + row) * q.sm : ((q.row0 + row) / q.V) * q.sn + ((q.row0 + row) % q.V) * q.sm;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
-#pragma unroll(WIDE ? 4 : 1)
+#pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
                     uint32_t r[32];
@@ -518,7 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     umma::tmem_ld_wait();
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + (WIDE ? run_sums[WIDE ? c + j : 0] : 0.f);
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + (several ? run_sums[c + j] : 0.f);
                     const int col = col0 + c;
                     if (add && live) {
 #pragma unroll
