@@ -200,11 +200,13 @@ MSD_API int msd_block_backward_plan(int dtype, const msd_tensor_t *result, const
  * logits, the log-probabilities and their gradients, `labels` floats per voxel each.  Here
  *   z[t,o] = bias[o] + sum_c weight[o,c] x[t,c],  lse[t] = log sum_o exp z[t,o],
  *   loss[t] = lse[t] - z[t,target[t]]
- * is formed tile by tile and only lse is kept.  A token t = n * voxels + v is one voxel
+ * is formed tile by tile and only lse is kept (in 48 bits, for tokens that are sure of their label).  A token t = n * voxels + v is one voxel
  * of `x` (element (n, c, v) at data[n*stride_batch + c*stride_channel + v*stride_voxel]:
  * images, volumes, and with batch 1 or voxels 1 the rows of a matrix).  dtype MSD_F32,
- * MSD_BF16 or MSD_F16 is the type of x, weight, bias and their gradients; sums, lse and the
- * loss are float32.  `weight` is dense [labels, channels], `bias` dense [labels] or NULL,
+ * MSD_BF16 or MSD_F16 is the type of x, weight, bias and their gradients; sums and the loss are
+ * float32.  In the products of 16-bit inputs the loss's gradient with respect to z is rounded to 16 bits too
+ * (not with at most 16 labels over voxels side by side; MSD_F16: in units of 2^-14 of the upstream
+ * gradient, and not at all with MSD_REDUCE_NONE).  `weight` is dense [labels, channels], `bias` dense [labels] or NULL,
  * `target` dense [batch * voxels].  A token whose target is `ignore_index` counts nowhere: its
  * features may hold anything.  A target that is neither ignore_index nor in [0, labels) makes
  * the loss, and every gradient its token reaches, NaN. */
@@ -276,7 +278,8 @@ typedef struct msd_span {
 MSD_API size_t msd_grad_norm_workspace_bytes(int64_t count);
 
 /* norm32 / norm64 (device, either may be NULL) = (sum of squares over all tensors)^(1/2), or the
- * largest magnitude; 0 without values.  Sums are float64 and have a fixed order. */
+ * largest magnitude; 0 without values.  Squares of 32 bytes are added in float32 (float64 tensors:
+ * float64), their sums in float64, in a fixed order: the norm is off by at most 3 2^-24. */
 MSD_API int msd_grad_norm(const msd_span_t *tensors, int64_t count, int norm_type, float *norm32, double *norm64,
                           void *workspace, size_t workspace_bytes, int device, void *stream);
 

@@ -111,13 +111,6 @@ __device__ __forceinline__ void bulk_g2s(void *dst_smem, const void *src_gmem, u
 
 // Tiled TMA loads (no multicast).  Coordinates are innermost first.  The innermost
 // coordinate times the element size must be a multiple of 16 bytes.
-__device__ __forceinline__ void tensor_g2s_3d(void *dst_smem, const CUtensorMap *map, int c0, int c1, int c2, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-                     smem_u32(dst_smem)),
-                 "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-                 : "memory");
-}
-
 __device__ __forceinline__ void tensor_g2s_4d(void *dst_smem, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(

@@ -1,7 +1,8 @@
 // Thin inline-PTX wrappers for the sm_100a tensor-core path (tcgen05): tensor-memory
-// allocation, shared-memory matrix descriptors, the TF32 MMA with its accumulator in tensor
-// memory, commit-to-mbarrier, and tensor-memory loads.  Single-CTA forms only
-// (cta_group::1); no cluster multicast is used anywhere.
+// allocation, shared-memory matrix descriptors, the TF32 and 16-bit MMAs with their accumulators in
+// tensor memory, commit-to-mbarrier, and tensor-memory loads.  TF32 in the single-CTA form
+// (cta_group::1), 16 bits for a pair of CTAs (cta_group::2), whose commit signals both of them.  No
+// load is a multicast.
 #pragma once
 #include <stdint.h>
 #include "tma.cuh"
@@ -68,15 +69,6 @@ __device__ __forceinline__ void mma_tf32(uint32_t d_tmem, uint64_t a_desc, uint6
 __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int m, int n, bool a_mn_major, bool b_mn_major) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
 }
 
 // Arrives (count 1) on `bar` once every MMA issued so far by this thread has completed;

@@ -1,7 +1,7 @@
 // Linear layer + softmax cross entropy: host side, the kernels around the products of
 // xent_mma.cuh, and the C entry points.  See xent.h for the formulas.
 //
-// forward   pack x (and W) -> kLse -> combine (lse, loss per token) -> finish (the reduction)
+// forward   pack x (and W) -> kLse -> combine (statistics, loss per token) -> finish (the reduction)
 // backward  pack x (and W) -> per piece of the labels: kGrad, column sums (db), kBack (dx, dW)
 #include <atomic>
 #include <string.h>

@@ -331,9 +331,9 @@ __global__ void __launch_bounds__(32 * kWarps, OP > 8 ? 1 : 2) narrow_kernel(con
     const int rows = (p.C + 3) / 4 * 4;
     float *ws = narrow_smem;                          // [rows][OP], zeros past the last channel
     float *bs = ws + rows * OP;                       // [OP]
-    float *gs = bs + OP;                              // [OP][128]
+    float *gs = bs + OP;                              // [OP][kVoxels]
     float *sums = gs + OP * kVoxels;     // [warp][groups][32]
-    int *keep = (int *)(((uintptr_t)(sums + WARPS * groups * 32) + 15) & ~(uintptr_t)15);  // [128]
+    int *keep = (int *)(((uintptr_t)(sums + WARPS * groups * 32) + 15) & ~(uintptr_t)15);  // [kVoxels]
     T *tiles = (T *)(keep + kVoxels);
     const int tile_elements = p.C * kRow;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;

@@ -164,7 +164,7 @@ def _empty_gradient(x, x_geometry):
 
 
 def capturing(x):
-    """Whether this thread's work on the device of ``x`` is being captured into a graph."""
+    """Whether work on the current stream, and so on ``x``, is being captured into a graph."""
     return x.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
@@ -256,9 +256,13 @@ def linear_cross_entropy(input, weight, bias, target, ignore_index=-100, reducti
     gradients, whatever its features hold.  ``reduction``: "mean" (over the tokens that count),
     "sum" or "none".
 
-    The loss is float32 for every input type (products of bfloat16 and float16 values are exact,
-    sums, exponentials and logarithms are float32).  Gradients have their tensors' types and are
-    the same bits in every run.  As in ``torch.nn.functional.cross_entropy`` a mean over no tokens is
+    The loss is float32 for every input type: products of bfloat16 and float16 values are exact, those of
+    float32 values are off by less than their own rounding (magnitudes below 1e-32 count as up to 2^-126 less),
+    sums, exponentials and logarithms are float32.  Gradients have their tensors' types and are the
+    same bits in every run.  With bfloat16 and float16 features the softmax gradient of a token
+    (probability minus one for its label) is rounded to that type before it is multiplied with weight and
+    features, unless there are at most 16 labels over images or volumes; float16 holds it down to 2^-38 of the
+    upstream gradient, and in three pieces of 8 bits for reduction "none".  As in ``torch.nn.functional.cross_entropy`` a mean over no tokens is
     NaN; a target that names no label makes the loss and the gradients that its token reaches NaN
     instead of ending the process."""
     _check(input, weight, bias, target, reduction)
