@@ -569,6 +569,7 @@ int forward(const Problem &p, float *loss, float *saved, void *ws, size_t wsb, i
         XENT_TRY(logit_product(p, q, op, n, 0, q.O, pairs, &m.p[0]));
         m.part = f.part, m.zy = f.zy;
         const int64_t tiles = (int64_t)m.p[0].tiles_m * m.p[0].tiles_n;
+        m.sum_blocks = !saved && tiles <= pairs ? kSumSmall : kSumStep;
         XENT_TRY(launch_mma<kLse>(m, q.P, (int)(tiles < pairs ? tiles : pairs), s));
         // many lanes per token where there are few tokens: their pairs would be joined one after the other
         const int slots = 2 * m.p[0].tiles_n;
@@ -629,7 +630,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     MmaParams m;
     XENT_TRY(common_params(p, q, op, t0, device, &m));
     XENT_TRY(logit_product(p, q, op, T_, o0, n, pairs, &m.p[0]));
-    m.label0 = (int)o0;
+    m.label0 = (int)o0, m.sum_blocks = kSumStep;
     m.stats = stats.at(t0), m.row_factor = row_factor ? row_factor + t0 : nullptr, m.factor = factor;
     m.columns = db ? b.columns : nullptr;
     m.g = b.g, m.g_width = gw, m.g_piece = g_piece;
@@ -674,6 +675,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
         r.vec = r.sc == 1 && ((uintptr_t)r.out & 15) == 0 && r.N % e == 0 && r.sm % e == 0 && r.sn % e == 0;
         if ((int64_t)r.tiles_m * r.tiles_n * r.splits > 0x7fffffff) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: %d x %d gradients are too many", r.M, r.N);
     }
+    m.sum_blocks = kSumBack;
     assign(&m, pairs, dx != nullptr, dw != nullptr);
     XENT_TRY(launch_mma<kBack>(m, q.P, pairs, s));
     for (int i = 0; i < 2; ++i)

@@ -17,9 +17,10 @@
 // drifts towards zero (a loss of 16-bit rows of 65536 channels: 4e-5 off, of 1000 channels 4e-7; a
 // rounding sum 1e-7).  So every stretch of the contraction is a sum of its own, small products first,
 // and the epilogue warps add these sums in registers (rounding to nearest), under the products of the next.
-// Float32 inputs: 64 at a time.  16-bit inputs: 1024 in logits, whatever their number (5e-7; 512 at a
-// time: 2.5e-7 and 6 % of a step of 4096 x 32768 x 1024, whose G has no time left for it), 4096 in
-// gradients, which are rounded to 16 bits.
+// Float32 inputs: 64 at a time.  16-bit inputs: 1024 in logits, the same ones forward and backward (5e-7 at
+// any length; 512 at a time: 2.5e-7 and 6 % of a step of 4096 x 32768 x 1024, whose G has no time left for
+// it; 256 at a time: 1.3e-7, 20 % of the loss alone), and 256 for a loss alone of one tile per pair or less, where it
+// costs nothing; 4096 in gradients, which are rounded to 16 bits.
 //
 // Two CTAs on neighbouring SMs work as a pair (cta_group::2) on tiles of 256 x 256: each loads its own
 // 128 rows of A and half of B, 32 KB per 64 of the contraction: 64 bytes per clock at the tensor core's
@@ -52,8 +53,8 @@ static_assert(kRegsIssue * 128 + kRegsEpilogue * 256 <= kRegsLaunch * kMmaThread
 
 enum Use { kLse = 0, kGrad = 1, kBack = 2 };
 
-// Blocks of 64 of the contraction whose products are added in the tensor core.
-__host__ __device__ constexpr int sum_blocks(int use, int pieces) { return pieces > 1 ? 1 : use == kBack ? 64 : 16; }
+// Blocks of 64 of the contraction whose products are added in the tensor core (powers of two).
+constexpr int kSumSmall = 4, kSumStep = 16, kSumBack = 64;
 __host__ __device__ constexpr int stages_of(int pieces) { return pieces == 1 ? 6 : 2; }
 __host__ __device__ constexpr size_t mma_smem_bytes(int pieces) {
     return 1024 + (size_t)stages_of(pieces) * pieces * (kABytes + kBBytes) + 2 * kTileN * sizeof(float) + 8 * 32 * kTurn * sizeof(float) + 256;
@@ -88,6 +89,7 @@ struct Factor {
 struct MmaParams {
     Product p[2];  // kLse, kGrad: [0]; kBack: [0] = dx, [1] = dW
     bool bf16;     // operand type: bfloat16, else float16
+    int sum_blocks;  // one piece: one of these, else 1
     // kLse, kGrad
     const void *bias;
     int bias_type;
@@ -188,7 +190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
     using namespace tma;
     static_assert(P == 1 || P == 3, "operands as they are, or in three pieces");
     constexpr bool WIDE = P > 1;
-    constexpr int F = sum_blocks(USE, P);  // a power of two
+    const int F = WIDE ? 1 : p.sum_blocks;
     constexpr int S = stages_of(P);
     constexpr int kStage = P * (kABytes + kBBytes);
     extern __shared__ unsigned char xent_smem[];
@@ -274,7 +276,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 // 8192 bytes, 8 k at 1024, so 16 k = 2048 bytes.
                 const uint32_t a_step = q.a_mn ? 2048 / 16 : 32 / 16, b_step = q.b_mn ? 2048 / 16 : 32 / 16;
                 for (int kb = it.k0; kb < it.k1; ++kb) {
-                    const bool first = (kb - it.k0) % F == 0;
+                    const bool first = ((kb - it.k0) & (F - 1)) == 0;
                     if (first) {
                         wait_parity(acc_empty + acc, acc_phase ^ 1, abort_flag, p.status, 22);
                         __syncwarp();
@@ -286,7 +288,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     umma::fence_after_sync();
                     const uint32_t a = lo0 + (uint32_t)(stage * kStage) / 16, b = a + P * kABytes / 16;
                     const int steps = min(kDepth / 16, (K - kb * kDepth + 15) / 16);
-                    const bool sum_done = (kb - it.k0) % F == F - 1 || kb + 1 == it.k1;
+                    const bool sum_done = ((kb - it.k0) & (F - 1)) == F - 1 || kb + 1 == it.k1;
                     if (umma::elect_one()) {
                         // pieces whose orders add up to 2, then 1, then 0: the small products first
 #pragma unroll
@@ -317,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
         int acc = 0;
         uint32_t acc_phase = 0;
         int parity = 0, biases_of = -1;
-        float run_sums[kTileN / 2];  // sums of the contraction so far
+        float sums[kTileN / 2];  // of the contraction so far
         while (items.get(it)) {
             const Product &q = p.p[it.which];
             const int row = it.m * kTileM + (int)rank * kCtaM + quad * 32 + lane;  // token (kBack, dW: label)
@@ -332,31 +334,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 p.stats.read(row, lse, rest);
                 if (p.row_factor) upstream = p.row_factor[row];
             }
-            const bool several = WIDE || it.k1 - it.k0 > F;
-            if (several) {
-#pragma unroll
-                for (int j = 0; j < kTileN / 2; ++j) run_sums[j] = 0.f;
-                for (int kb = it.k0; kb + F < it.k1; kb += F) {
-                    wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 25);
-                    __syncwarp();
-                    umma::fence_after_sync();
-                    const uint32_t t = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
-#pragma unroll
-                    for (int c = 0; c < kTileN / 2; c += 32) {
-                        if (c >= cols) continue;
-                        uint32_t r[32];
-                        umma::tmem_ld32_issue(t + c, r);
-                        umma::tmem_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) run_sums[c + j] += __uint_as_float(r[j]);
-                    }
-                    umma::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) umma::arrive_at(umma::map_rank(smem_u32(acc_empty + acc), 0));
-                    if (++acc == 2) acc = 0, acc_phase ^= 1;
-                }
-            }
-            const uint32_t t0 = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
             if (USE != kBack && it.n != biases_of) {
                 // this half's biases; labels past the end count as -infinity
                 biases_of = it.n, parity ^= 1;
@@ -366,9 +343,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 named_barrier(1 + half, 128);
             }
             const float *bias_h = bias_s + parity * kTileN + half * (kTileN / 2);
-            wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 24);
-            __syncwarp();
-            umma::fence_after_sync();
+            // The tile's sums go to registers and leave the tensor memory to the next products at once: with the
+            // arithmetic below in between, the products of the next tile would wait for it.
+#pragma unroll
+            for (int j = 0; j < kTileN / 2; ++j) sums[j] = 0.f;
+            for (int kb = it.k0; kb < it.k1; kb += F) {
+                wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 24);
+                __syncwarp();
+                umma::fence_after_sync();
+                const uint32_t t = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                for (int c = 0; c < kTileN / 2; c += 32) {
+                    if (c >= cols) continue;
+                    uint32_t r[32];
+                    umma::tmem_ld32_issue(t + c, r);
+                    umma::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sums[c + j] += __uint_as_float(r[j]);
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) umma::arrive_at(umma::map_rank(smem_u32(acc_empty + acc), 0));
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
+            }
             if (USE == kLse) {
                 float top = -CUDART_INF_F, sum = 0.f;
                 const bool live = in;
@@ -376,14 +373,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
-                    uint32_t r[32];
-                    __syncwarp();
-                    umma::tmem_ld32_issue(t0 + c, r);
-                    umma::tmem_ld_wait();
-                    if (several) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[c + j]);
-                    }
                     float z[32], m = -CUDART_INF_F;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
@@ -391,8 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                         const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float v = __uint_as_float(r[j + i]);
-                            z[j + i] = v + bb[i];
+                            z[j + i] = sums[c + j + i] + bb[i];
                         }
                     }
                     if (c + 32 > cols) {  // columns that no product wrote
@@ -427,14 +415,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= stored) continue;
-                    uint32_t r[32];
-                    __syncwarp();
-                    umma::tmem_ld32_issue(t0 + c, r);
-                    umma::tmem_ld_wait();
-                    if (several) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + run_sums[c + j]);
-                    }
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
@@ -442,8 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                         const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float a = __uint_as_float(r[j + i]);
-                            v[j + i] = (a + bb[i]) - lse - rest;
+                            v[j + i] = (sums[c + j + i] + bb[i]) - lse - rest;
                         }
                     }
                     float d = 0.f;  // p - 1 of the target: exact where p is close to 1
@@ -519,13 +498,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
 #pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
-                    uint32_t r[32];
-                    __syncwarp();
-                    umma::tmem_ld32_issue(t0 + c, r);
-                    umma::tmem_ld_wait();
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + (several ? run_sums[c + j] : 0.f);
+                    for (int j = 0; j < 32; ++j) v[j] = sums[c + j];
                     const int col = col0 + c;
                     if (add && live) {
 #pragma unroll
@@ -608,10 +583,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     }
                 }
             }
-            umma::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) umma::arrive_at(umma::map_rank(smem_u32(acc_empty + acc), 0));
-            if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
     }
     umma::fence_before_sync();

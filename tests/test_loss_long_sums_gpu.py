@@ -29,3 +29,21 @@ def test_long_contraction(cuda_device, T, C, O, dtype):
         each = linear_cross_entropy(*leaves, None, y, reduction="none").detach().double()
         assert bool(((each - want).abs() <= bound).all())
     assert _lib.device_status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("T,C,O", [(61, 1000, 5003), (300, 8192, 1000), (150, 65536, 500)])
+def test_small_loss_alone(cuda_device, T, C, O, dtype):
+    """Logits have standard deviation 2, a stretch of 256 products 2 / sqrt(n) with n = C / 256.  Its 16 additions
+    truncate by half a step, 2^-24 of the partial sum, in the mean: at most 16 x 2^-24 x 2 / sqrt(n) per stretch, and as
+    the stretches' signs are random 2^-19 for all n of them, whatever n.  Losses are 9 in the mean: 2^-22 of them."""
+    from msd_pytorch_b200 import linear_cross_entropy
+
+    g = torch.Generator(device=cuda_device).manual_seed(C + 1)
+    x = torch.randn(T, C, device=cuda_device, generator=g).to(dtype)
+    w = (torch.randn(O, C, device=cuda_device, generator=g) * (2 / C ** 0.5)).to(dtype)
+    y = torch.randint(0, O, (T,), device=cuda_device, generator=g)
+    want = torch.nn.functional.cross_entropy(x.double() @ w.double().t(), y, reduction="none")
+    with torch.no_grad():
+        each = linear_cross_entropy(x, w, None, y, reduction="none").double()
+    assert float((each - want).norm()) <= 2.0 ** -22 * float(want.norm())
