@@ -14,6 +14,12 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long-running test")
 
 
+def pytest_collection_modifyitems(items):
+    """Comparisons with the reference's own build, which exists only where its checkout does, come last: a run
+    that stops at the first failure reaches everything else before them."""
+    items.sort(key=lambda item: item.fspath.basename == "test_parity_configs_gpu.py")
+
+
 @pytest.fixture(scope="session")
 def cuda_device():
     import torch
