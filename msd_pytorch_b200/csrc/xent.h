@@ -21,7 +21,7 @@
 namespace msd {
 namespace xent {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Features {  // x or dx: element (n, c, v) at data[n*sn + c*sc + v*sv]; token = n*V + v
     void *p;

@@ -35,6 +35,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
+#include "f32x2.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 #include "xent.h"
@@ -319,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
         int acc = 0;
         uint32_t acc_phase = 0;
         int parity = 0, biases_of = -1;
-        float sums[kTileN / 2];  // of the contraction so far
+        Pair sums[kTileN / 4];  // of the contraction so far
         while (items.get(it)) {
             const Product &q = p.p[it.which];
             const int row = it.m * kTileM + (int)rank * kCtaM + quad * 32 + lane;  // token (kBack, dW: label)
@@ -346,7 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
             // The tile's sums go to registers and leave the tensor memory to the next products at once: with the
             // arithmetic below in between, the products of the next tile would wait for it.
 #pragma unroll
-            for (int j = 0; j < kTileN / 2; ++j) sums[j] = 0.f;
+            for (int j = 0; j < kTileN / 4; ++j) sums[j] = pair(0.f, 0.f);
             for (int kb = it.k0; kb < it.k1; kb += F) {
                 wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 24);
                 __syncwarp();
@@ -359,7 +360,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     umma::tmem_ld32_issue(t + c, r);
                     umma::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sums[c + j] += __uint_as_float(r[j]);
+                    for (int j = 0; j < 16; ++j) sums[c / 2 + j] = add2(sums[c / 2 + j], pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
                 }
                 umma::fence_before_sync();
                 __syncwarp();
@@ -375,13 +376,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     if (c >= cols) continue;
                     float z[32], m = -CUDART_INF_F;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 b4 = *reinterpret_cast<const float4 *>(bias_h + c + j);
-                        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            z[j + i] = sums[c + j + i] + bb[i];
-                        }
+                    for (int j = 0; j < 16; j += 2) {
+                        const ulonglong2 b4 = *reinterpret_cast<const ulonglong2 *>(bias_h + c + 2 * j);
+                        unpair(add2(sums[c / 2 + j], b4.x), z[2 * j], z[2 * j + 1]);
+                        unpair(add2(sums[c / 2 + j + 1], b4.y), z[2 * j + 2], z[2 * j + 3]);
                     }
                     if (c + 32 > cols) {  // columns that no product wrote
 #pragma unroll
@@ -397,10 +395,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     }
                     const float up = fmaxf(top, m);
                     const float base = up == -CUDART_INF_F ? 0.f : up;
-                    float s[4] = {0.f, 0.f, 0.f, 0.f};
+                    Pair s[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                    const Pair off = pair(-base, -base), scale = pair(kLog2e, kLog2e);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast((z[j] - base) * kLog2e);  // a NaN logit makes the sum NaN
-                    sum = sum * exp2_fast((top - base) * kLog2e) + ((s[0] + s[1]) + (s[2] + s[3]));
+                    for (int j = 0; j < 16; ++j) {
+                        float e0, e1;
+                        unpair(mul2(add2(pair(z[2 * j], z[2 * j + 1]), off), scale), e0, e1);
+                        s[j & 1] = add2(s[j & 1], pair(exp2_fast(e0), exp2_fast(e1)));  // a NaN logit makes the sum NaN
+                    }
+                    float s0, s1;
+                    unpair(add2(s[0], s[1]), s0, s1);
+                    sum = sum * exp2_fast((top - base) * kLog2e) + (s0 + s1);
                     top = up;
                 }
                 if (live && !*abort_flag) p.part[(int64_t)(2 * it.n + half) * q.M + row] = make_float2(top, sum);
@@ -408,39 +413,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 const bool live = in, counts = live && y != p.ignore;
                 float g = counts ? upstream * p.g_scale : 0.f;
                 if (counts && (y < 0 || y >= p.labels)) g = CUDART_NAN_F;
-                const int hit = y >= p.label0 + col0 && y < p.label0 + col0 + cols ? (int)(y - p.label0 - col0) : -1;
+                const int hit = counts && y >= p.label0 + col0 && y < p.label0 + col0 + cols ? (int)(y - p.label0 - col0) : -1;
+                const bool all_count = __all_sync(0xffffffffu, counts);
+                const Pair off = pair(-lse, -lse), off_rest = pair(rest * -kLog2e, rest * -kLog2e), scale = pair(kLog2e, kLog2e), factor = pair(g, g);
                 const int stored = (int)min((int64_t)width, p.g_width - col0);
                 const bool ok = !*abort_flag;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
 #pragma unroll
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= stored) continue;
-                    float v[32];
+                    float v[32];  // log2 p
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 b4 = *reinterpret_cast<const float4 *>(bias_h + c + j);
-                        const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            v[j + i] = (sums[c + j + i] + bb[i]) - lse - rest;
-                        }
+                    for (int j = 0; j < 16; j += 2) {
+                        const ulonglong2 b4 = *reinterpret_cast<const ulonglong2 *>(bias_h + c + 2 * j);
+                        unpair(fma2(add2(add2(sums[c / 2 + j], b4.x), off), scale, off_rest), v[2 * j], v[2 * j + 1]);
+                        unpair(fma2(add2(add2(sums[c / 2 + j + 1], b4.y), off), scale, off_rest), v[2 * j + 2], v[2 * j + 3]);
                     }
                     float d = 0.f;  // p - 1 of the target: exact where p is close to 1
                     const bool any = __any_sync(0xffffffffu, hit >= c && hit < c + 32);
                     if (any) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) d = hit == c + j ? v[j] : d;
-                        d = expm1f(d);
+                        d = expm1f(d * kLn2);
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j] * kLog2e);
+                    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j]);
                     if (any) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = hit == c + j ? d : v[j];
                     }
-                    // columns past the last label and ignored tokens are exact zeros whatever the logits hold
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = counts && c + j < cols ? v[j] * g : 0.f;
+                    for (int j = 0; j < 16; ++j) unpair(mul2(pair(v[2 * j], v[2 * j + 1]), factor), v[2 * j], v[2 * j + 1]);
+                    if (c + 32 > cols || !all_count) {  // past the last label, and ignored tokens: exact zeros whatever the logits hold
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = counts && c + j < cols ? v[j] : 0.f;
+                    }
                     // A lane has 64 bytes of its row.  Stored like that, every store touches 32 rows (292 us for
                     // 4096 x 32768 x 1024, 207 without the stores); turned in shared memory, it writes whole
                     // 64-byte pieces of 8 rows (229).
@@ -500,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                     if (c >= cols) continue;
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = sums[c + j];
+                    for (int j = 0; j < 16; ++j) unpair(sums[c / 2 + j], v[2 * j], v[2 * j + 1]);
                     const int col = col0 + c;
                     if (add && live) {
 #pragma unroll
