@@ -19,7 +19,7 @@ namespace xent {
 
 constexpr int kThreads = 256;
 constexpr int kCombineBlocks = 592;
-constexpr int64_t kPieceBytes = 256ll << 20;  // G held at a time (half as much again where that saves a piece)
+constexpr int64_t kPieceBytes = 256ll << 20;  // G held at a time (half as much again where that saves a piece or a chunk)
 constexpr int64_t kPieceLabels = 256;         // labels of a piece, at least (fewer only if there are no more)
 constexpr int64_t kChunkBytes = 512ll << 20;  // packed features held at a time
 
@@ -302,6 +302,7 @@ static Plan make_plan(const Problem &p, bool backward) {
     const int64_t g_labels = q.O < kPieceLabels ? round_up(q.O, 64) : kPieceLabels;
     const int64_t by_x = kChunkBytes / (2 * q.P * q.ld), by_g = kPieceBytes / (2 * q.P * g_labels);
     q.chunk = (by_x < by_g ? by_x : by_g) / kTileM * kTileM;
+    if (q.T <= by_g + by_g / 2 && q.T <= by_x) q.chunk = q.T;
     if (q.chunk < 16 * kTileM) q.chunk = 16 * kTileM;
     if (q.chunk > q.T) q.chunk = q.T;
     q.chunks = q.T ? ceil_div(q.T, q.chunk) : 0;
@@ -477,18 +478,21 @@ static int pack_operands(const Problem &p, const Plan &q, const Operands &op, in
 }
 
 template <int USE>
-static int launch_mma(const MmaParams &m, int P, int pairs, cudaStream_t s) {
-    auto kern = P > 1 ? xent_mma_kernel<USE, 3> : xent_mma_kernel<USE, 1>;
+static int launch_mma(const MmaParams &m, int P, bool run, int pairs, cudaStream_t s) {
+    const int which = P > 1 ? 2 : run;
+    auto kern = which == 2 ? xent_mma_kernel<USE, 3, true> : which ? xent_mma_kernel<USE, 1, true> : xent_mma_kernel<USE, 1, false>;
     const size_t smem = mma_smem_bytes(P);
-    static std::atomic<uint64_t> ready[2];  // devices whose kernel is set up, for one piece and for three
+    static std::atomic<uint64_t> ready[3];  // devices whose kernel is set up
     int device = 0;
     MSD_CUDA_TRY(cudaGetDevice(&device));
-    if (device >= 64 || !(ready[P > 1].load() >> device & 1)) {
-        cudaFuncAttributes a;
-        MSD_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
-        if (a.numRegs < kRegsLaunch) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: built with %d registers per thread, %d expected", a.numRegs, kRegsLaunch);
+    if (device >= 64 || !(ready[which].load() >> device & 1)) {
+        if (which) {
+            cudaFuncAttributes a;
+            MSD_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
+            if (a.numRegs < kRegsLaunch) MSD_FAIL(MSD_ERR_UNSUPPORTED, "linear cross entropy: built with %d registers per thread, %d expected", a.numRegs, kRegsLaunch);
+        }
         MSD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        if (device < 64) ready[P > 1].fetch_or(1ull << device);
+        if (device < 64) ready[which].fetch_or(1ull << device);
     }
     kern<<<2 * pairs, kMmaThreads, smem, s>>>(m);
     return launched();
@@ -570,7 +574,7 @@ int forward(const Problem &p, float *loss, float *saved, void *ws, size_t wsb, i
         m.part = f.part, m.zy = f.zy;
         const int64_t tiles = (int64_t)m.p[0].tiles_m * m.p[0].tiles_n;
         m.sum_blocks = !saved && tiles <= pairs ? kSumSmall : kSumStep;
-        XENT_TRY(launch_mma<kLse>(m, q.P, (int)(tiles < pairs ? tiles : pairs), s));
+        XENT_TRY(launch_mma<kLse>(m, q.P, m.p[0].k_blocks > m.sum_blocks, (int)(tiles < pairs ? tiles : pairs), s));
         // many lanes per token where there are few tokens: their pairs would be joined one after the other
         const int slots = 2 * m.p[0].tiles_n;
         alone = q.chunks == 1 && n * slots <= 8192;  // one block's work is less than a launch
@@ -637,7 +641,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     // |G| <= 2 in units of the factor: one float16 holds it times 2^14, down to 2^-38
     m.g_scale = p.dtype == MSD_F16 && q.P == 1 ? 16384.f : 1.f;
     const int64_t tiles = (int64_t)m.p[0].tiles_m * m.p[0].tiles_n;
-    XENT_TRY(launch_mma<kGrad>(m, q.P, (int)(tiles < pairs ? tiles : pairs), s));
+    XENT_TRY(launch_mma<kGrad>(m, q.P, m.p[0].k_blocks > m.sum_blocks, (int)(tiles < pairs ? tiles : pairs), s));
     if (db) {
         const int x = n < 1024 ? 8 : 32;  // few labels: more lanes for each
         auto sum = x == 8 ? column_sum_kernel<8> : column_sum_kernel<32>;
@@ -677,7 +681,7 @@ static int backward_piece(const Problem &p, const Plan &q, const Operands &op, c
     }
     m.sum_blocks = kSumBack;
     assign(&m, pairs, dx != nullptr, dw != nullptr);
-    XENT_TRY(launch_mma<kBack>(m, q.P, pairs, s));
+    XENT_TRY(launch_mma<kBack>(m, q.P, (dx && ceil_div(X.k_blocks, X.splits) > kSumBack) || (dw && ceil_div(W.k_blocks, W.splits) > kSumBack), pairs, s));
     for (int i = 0; i < 2; ++i)
         if (m.p[i].parts && (i == 0 ? dx != nullptr : dw != nullptr)) {
             join_kernel<<<(unsigned)ceil_div((int64_t)m.p[i].M * m.p[i].N, m.p[i].splits <= kFewSplits ? kThreads : 32), kThreads, 0, s>>>(m, i, p.dtype);

@@ -20,7 +20,7 @@
 // Float32 inputs: 64 at a time.  16-bit inputs: 1024 in logits, the same ones forward and backward (5e-7 at
 // any length; 512 at a time: 2.5e-7 and 6 % of a step of 4096 x 32768 x 1024, whose G has no time left for
 // it; 256 at a time: 1.3e-7, 20 % of the loss alone), and 256 for a loss alone of one tile per pair or less, where it
-// costs nothing; 4096 in gradients, which are rounded to 16 bits.
+// costs nothing; 65536 in gradients (8e-6), which are rounded to 16 bits.
 //
 // Two CTAs on neighbouring SMs work as a pair (cta_group::2) on tiles of 256 x 256: each loads its own
 // 128 rows of A and half of B, 32 KB per 64 of the contraction: 64 bytes per clock at the tensor core's
@@ -55,7 +55,7 @@ static_assert(kRegsIssue * 128 + kRegsEpilogue * 256 <= kRegsLaunch * kMmaThread
 enum Use { kLse = 0, kGrad = 1, kBack = 2 };
 
 // Blocks of 64 of the contraction whose products are added in the tensor core (powers of two).
-constexpr int kSumSmall = 4, kSumStep = 16, kSumBack = 64;
+constexpr int kSumSmall = 4, kSumStep = 16, kSumBack = 1024;
 __host__ __device__ constexpr int stages_of(int pieces) { return pieces == 1 ? 6 : 2; }
 __host__ __device__ constexpr size_t mma_smem_bytes(int pieces) {
     return 1024 + (size_t)stages_of(pieces) * pieces * (kABytes + kBBytes) + 2 * kTileN * sizeof(float) + 8 * 32 * kTurn * sizeof(float) + 256;
@@ -186,12 +186,13 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-template <int USE, int P>
+// RUN: the contraction of a tile may be several sums, which are added in registers.
+template <int USE, int P, bool RUN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent_mma_kernel(const __grid_constant__ MmaParams p) {
     using namespace tma;
-    static_assert(P == 1 || P == 3, "operands as they are, or in three pieces");
+    static_assert(P == 1 || (P == 3 && RUN), "operands as they are, or in three pieces");
     constexpr bool WIDE = P > 1;
-    const int F = WIDE ? 1 : p.sum_blocks;
+    const int F = WIDE ? 1 : RUN ? p.sum_blocks : 1 << 30;
     constexpr int S = stages_of(P);
     constexpr int kStage = P * (kABytes + kBBytes);
     extern __shared__ unsigned char xent_smem[];
@@ -214,10 +215,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
     umma::cluster_sync();  // both CTAs' barriers exist from here on
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    // Three pieces: the epilogue warps keep 128 sums per thread.  kRegsIssue x 128 + kRegsEpilogue x 256 is
+    // The epilogue warps keep 128 sums per thread.  kRegsIssue x 128 + kRegsEpilogue x 256 is
     // what the block was launched with (kRegsLaunch x 384; the launcher checks the compiled kernel).
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // The loops of both issuing warps run with all lanes (see umma::elect_one): with one lane in a
         // branch of its own the products of 64 took 1000 clocks to issue instead of the 512 they run.
         if (warp == 0) {
@@ -313,14 +314,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+        if (RUN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         const int half = (warp - 4) >> 2, quad = warp & 3;
         Items<USE> items(p);
         Item it;
         int acc = 0;
         uint32_t acc_phase = 0;
         int parity = 0, biases_of = -1;
-        Pair sums[kTileN / 4];  // of the contraction so far
+        Pair sums[RUN ? kTileN / 4 : 1];  // of the contraction so far
         while (items.get(it)) {
             const Product &q = p.p[it.which];
             const int row = it.m * kTileM + (int)rank * kCtaM + quad * 32 + lane;  // token (kBack, dW: label)
@@ -344,42 +345,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 named_barrier(1 + half, 128);
             }
             const float *bias_h = bias_s + parity * kTileN + half * (kTileN / 2);
-            // The tile's sums go to registers and leave the tensor memory to the next products at once: with the
-            // arithmetic below in between, the products of the next tile would wait for it.
+            uint32_t t0 = 0;  // the tile in tensor memory, unless its sums are in registers
+            if constexpr (RUN) {
+                // They leave the tensor memory to the next products at once: with the arithmetic below in
+                // between, the products of the next tile would wait for it.
 #pragma unroll
-            for (int j = 0; j < kTileN / 4; ++j) sums[j] = pair(0.f, 0.f);
-            for (int kb = it.k0; kb < it.k1; kb += F) {
+                for (int j = 0; j < kTileN / 4; ++j) sums[j] = pair(0.f, 0.f);
+                for (int kb = it.k0; kb < it.k1; kb += F) {
+                    wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 24);
+                    __syncwarp();
+                    umma::fence_after_sync();
+                    const uint32_t t = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                    for (int c = 0; c < kTileN / 2; c += 32) {
+                        if (c >= cols) continue;
+                        uint32_t r[32];
+                        umma::tmem_ld32_issue(t + c, r);
+                        umma::tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sums[c / 2 + j] = add2(sums[c / 2 + j], pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+                    }
+                    umma::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) umma::arrive_at(umma::map_rank(smem_u32(acc_empty + acc), 0));
+                    if (++acc == 2) acc = 0, acc_phase ^= 1;
+                }
+            } else {
                 wait_parity(acc_full + acc, acc_phase, abort_flag, p.status, 24);
                 __syncwarp();
                 umma::fence_after_sync();
-                const uint32_t t = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
+                t0 = tmem + acc * kTileN + half * width + ((uint32_t)(quad * 32) << 16);
+            }
+            // Columns [c, c + 32) of this half.  From tensor memory in a loop of 32 columns: straight-line code for
+            // all of them runs once per tile and waits for its instructions (dx of 2 million voxels: 1150 us
+            // against 690).
+            const auto take = [&](int c, Pair (&x)[16]) {
+                if constexpr (RUN) {
 #pragma unroll
-                for (int c = 0; c < kTileN / 2; c += 32) {
-                    if (c >= cols) continue;
+                    for (int j = 0; j < 16; ++j) x[j] = sums[c / 2 + j];
+                } else {
                     uint32_t r[32];
-                    umma::tmem_ld32_issue(t + c, r);
+                    __syncwarp();
+                    umma::tmem_ld32_issue(t0 + c, r);
                     umma::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sums[c / 2 + j] = add2(sums[c / 2 + j], pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+                    for (int j = 0; j < 16; ++j) x[j] = pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
                 }
-                umma::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) umma::arrive_at(umma::map_rank(smem_u32(acc_empty + acc), 0));
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
-            }
+            };
             if (USE == kLse) {
                 float top = -CUDART_INF_F, sum = 0.f;
                 const bool live = in;
                 const int hit = live && y >= col0 && y < col0 + cols ? (int)(y - col0) : -1;
-#pragma unroll
+#pragma unroll(RUN ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
+                    Pair x[16];
+                    take(c, x);
                     float z[32], m = -CUDART_INF_F;
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const ulonglong2 b4 = *reinterpret_cast<const ulonglong2 *>(bias_h + c + 2 * j);
-                        unpair(add2(sums[c / 2 + j], b4.x), z[2 * j], z[2 * j + 1]);
-                        unpair(add2(sums[c / 2 + j + 1], b4.y), z[2 * j + 2], z[2 * j + 3]);
+                        unpair(add2(x[j], b4.x), z[2 * j], z[2 * j + 1]);
+                        unpair(add2(x[j + 1], b4.y), z[2 * j + 2], z[2 * j + 3]);
                     }
                     if (c + 32 > cols) {  // columns that no product wrote
 #pragma unroll
@@ -419,15 +446,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 const int stored = (int)min((int64_t)width, p.g_width - col0);
                 const bool ok = !*abort_flag;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
-#pragma unroll
+#pragma unroll(RUN ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= stored) continue;
+                    Pair x[16];
+                    take(c, x);
                     float v[32];  // log2 p
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const ulonglong2 b4 = *reinterpret_cast<const ulonglong2 *>(bias_h + c + 2 * j);
-                        unpair(fma2(add2(add2(sums[c / 2 + j], b4.x), off), scale, off_rest), v[2 * j], v[2 * j + 1]);
-                        unpair(fma2(add2(add2(sums[c / 2 + j + 1], b4.y), off), scale, off_rest), v[2 * j + 2], v[2 * j + 3]);
+                        unpair(fma2(add2(add2(x[j], b4.x), off), scale, off_rest), v[2 * j], v[2 * j + 1]);
+                        unpair(fma2(add2(add2(x[j + 1], b4.y), off), scale, off_rest), v[2 * j + 2], v[2 * j + 3]);
                     }
                     float d = 0.f;  // p - 1 of the target: exact where p is close to 1
                     const bool any = __any_sync(0xffffffffu, hit >= c && hit < c + 32);
@@ -502,12 +531,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                 const bool add = !split && q.add;
                 const int64_t at = q.linear ? (q.row0 + row) * q.sm : ((q.row0 + row) / q.V) * q.sn + ((q.row0 + row) % q.V) * q.sm;
                 float *turn = turn_s + (warp - 4) * 32 * kTurn;
-#pragma unroll
+#pragma unroll(RUN ? 4 : 1)
                 for (int c = 0; c < kTileN / 2; c += 32) {
                     if (c >= cols) continue;
+                    Pair x[16];
+                    take(c, x);
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) unpair(sums[c / 2 + j], v[2 * j], v[2 * j + 1]);
+                    for (int j = 0; j < 16; ++j) unpair(x[j], v[2 * j], v[2 * j + 1]);
                     const int col = col0 + c;
                     if (add && live) {
 #pragma unroll
@@ -589,6 +620,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1) xent
                         }
                     }
                 }
+            }
+            if constexpr (!RUN) {
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) umma::arrive_at(umma::map_rank(smem_u32(acc_empty + acc), 0));
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
             }
         }
     }
