@@ -25,8 +25,8 @@
 // Two CTAs on neighbouring SMs work as a pair (cta_group::2) on tiles of 256 x 256: each loads its own
 // 128 rows of A and half of B, 32 KB per 64 of the contraction: 64 bytes per clock at the tensor core's
 // rate, which is about what L2 delivers to an SM (128 x 256 tiles of one CTA: 96).  4096 x 32768 x 1024 in
-// bfloat16: kLse 173 us (1.59 PFLOP/s, tensor pipe 93 % busy), kBack 361 us for twice the products
-// (94 %), kGrad 220 us (69 %: its epilogue has a third more to do than the products leave time for).
+// bfloat16: kLse 169 us (1.63 PFLOP/s, tensor pipe 95 % busy), kBack 358 us for twice the products
+// (94 %), kGrad 220 us (70 %: its epilogue has a third more to do than the products leave time for).
 // The float32 accumulators (256 columns of a CTA's tensor memory) are double-buffered, so that the
 // epilogue of one tile runs under the products of the next.  Warp 0 issues the TMA loads, one thread of
 // rank 0's warp 1 the products of the pair, warps 4..11 the epilogue (warp % 4 = the 32 rows it may

@@ -82,6 +82,10 @@ static int narrow_stages(const Problem &p) {
     return n > 4 ? 4 : (int)n;
 }
 
+// Where both can: two 1024 x 1024 images of 101 float32 channels, loss and gradients of 4, 8 and 16 labels 430, 600
+// and 1100 us here and 3900 to 4000 as tensor-core products (tiles of 128 labels at least); one of 256 x 256, 51
+// channels, 40, 44 and 51 against 138.  bfloat16, 16 labels: 1660 against 2830 us, and with 160 channels, the
+// worst found, 395 against 370.
 bool narrow_supported(const Problem &p) {
     return p.labels <= kNarrowLabels && p.x.sv == 1 && p.x.V >= kVoxels && p.x.C <= 1024 && p.x.N > 0 && narrow_stages(p) >= 1;
 }
@@ -182,7 +186,7 @@ static int launch_grad_kernel(const NarrowParams &q, size_t smem, int device, in
 template <typename T, int OP, bool ALIGNED>
 static int launch_grad(const NarrowParams &q, int device, int *blocks, cudaStream_t s) {
     const size_t smem = narrow_fixed_bytes(q.C, OP) + q.stages * narrow_tile_bytes(q.C, sizeof(T)) + 16;
-    if constexpr (OP <= 4)  // sums of dW in registers: 64 of them
+    if constexpr (OP <= 4)  // sums of dW in registers: 64 of them (430 us for two 1024 x 1024 images of 101 channels, 465 without)
         if (q.C <= kRegisterChannels * kSlots) return launch_grad_kernel<narrow_kernel<T, OP, ALIGNED, true>>(q, smem, device, blocks, s);
     return launch_grad_kernel<narrow_kernel<T, OP, ALIGNED, false>>(q, smem, device, blocks, s);
 }
