@@ -10,8 +10,8 @@
 // 2^-27 |v| is left).  A product is a a' + (a b' + b a') + (a c' + b b' + c a'): what is dropped is below
 // 2^-25 of it, less than a float32 product's own rounding, and as the pieces have float32's range of exponents
 // this holds whatever the other values of the tensor are.  (Two float16 pieces under one power of two
-// per tensor need three products instead of six, but lose values 2^-24 below the tensor's largest step by
-// step: one token of 1e8 took 8 bits from all others.)
+// per tensor need three products instead of six, but hold nothing finer than 2^-39 of the tensor's largest
+// value: one token of 1e8 left 13 bits to values near 1.)
 //
 // The tensor core's float32 additions truncate: a sum of n of them is off by up to n 2^-23 and
 // drifts towards zero (a loss of 16-bit rows of 65536 channels: 4e-5 off, of 1000 channels 4e-7; a
